@@ -278,6 +278,112 @@ int xe_attn_decode_dev_static(xe_ctx *ctx, const float *q_dev,
 int xe_attn_splits(const xe_ctx *ctx, int batch, int hq, int hkv, int hd,
                    int max_ctx, int *merge_launch);
 
+/* ---- a KV cache in pages ----
+ * For callers that serve many streams from one pool of memory: the keys and
+ * values of a stream lie in pages of page_size positions, anywhere in the
+ * pool, in the order of its row of the page table.  No counterpart in the
+ * reference, whose caches are one block a stream.  All pointers are device
+ * memory, and the calls are asynchronous on the ctx stream: nothing is
+ * allocated in the append, and the attention's workspace belongs to the ctx
+ * and grows with the first calls.
+ *
+ * An entry of the table outside [0, n_pages) is no page: its positions hold
+ * no keys (pages of a sliding window that were given back, for instance). */
+typedef struct xe_paged_kv {
+  uint16_t *k, *v;       /* bf16; row (page, kv head h, slot) of hd elements at
+                            page * page_stride + (h * page_size + slot) * hd;
+                            16-byte aligned */
+  const int32_t *table;  /* [batch, max_pages] pages of each stream */
+  uint64_t page_stride;  /* elements from page to page, a multiple of 8 (a pool
+                            that interleaves layers); 0: hkv * page_size * hd */
+  int n_pages;           /* pages of k and of v */
+  int hkv;               /* key/value heads */
+  int page_size;         /* positions a page: a power of two, 16..1024 */
+  int hd;                /* 64, 128 or 256 */
+  int batch;             /* streams, 1..4096 */
+  int max_pages;         /* table entries a stream; max_pages * page_size <=
+                            2^30 */
+} xe_paged_kv;
+
+/* New tokens' rows of xe_paged_append_dev, fp32.  Row i belongs to the stream
+ * b with start[b] <= i < start[b + 1] and to position pos[b] + i - start[b];
+ * start null: one row a stream, row b at pos[b] (n_rows = batch). */
+typedef struct xe_paged_rows {
+  const float *q, *k, *v;   /* q [n_rows, hq * hd] in rows of ldq (null: no
+                               queries), k and v [n_rows, hkv * hd] in rows of
+                               ldkv: the parts of a fused projection's rows */
+  uint64_t ldq, ldkv;       /* floats from row to row */
+  float *q_out;             /* [n_rows, hq * hd] in rows of ldqo; may be q */
+  uint64_t ldqo;
+  const int32_t *pos;       /* [batch] */
+  const int32_t *start;     /* [batch + 1], ascending, or null */
+  const float *q_norm_w, *k_norm_w; /* [hd] RMSNorm (1 + w) over each head of
+                               q / k before the rotation, or null */
+  const float *rope_cos, *rope_sin; /* [rope_len, hd / 2]: dimensions j and
+                               j + hd / 2 of q and k are rotated by the row of
+                               the position; null: no rotation */
+  float eps;
+  int rope_len;
+  int n_rows, hq;           /* hq is not read without q */
+} xe_paged_rows;
+
+/* Appends rows to the streams' pages, keys and values rounded to bf16 (RNE),
+ * and writes the queries, normalised and rotated, as fp32.  Left out, with
+ * none of its q, k and v written: a row behind start[batch] or before
+ * start[0], one whose position lies outside [0, max_pages * page_size) or
+ * [0, rope_len), one whose page the table does not have; streams with
+ * pos[b] < 0 take no rows.  Every other byte of the pages stays as it was.
+ * Streams that share a page (a common prefix) must not append to it: of two
+ * rows for one slot either may end up there, in part too. */
+int xe_paged_append_dev(xe_ctx *ctx, const xe_paged_kv *kv,
+                        const xe_paged_rows *rows);
+/* Attention of one query token a stream over its pages:
+ *   q    fp32 [batch, hq * hd] in rows of ldq floats (0: hq * hd)
+ *   lens int32 [batch]: tokens of the stream, the new one included
+ *   out  fp32 [batch, hq * hd] in rows of ldo floats (0: hq * hd)
+ * scores = (q . k) * scale; softmax over the positions [0, lens[b]), with
+ * window > 0 over the last `window` of them, of which the table has the page.
+ * Query head h reads kv head h / (hq / hkv); hq is a multiple of hkv.  A
+ * stream with no such position (lens[b] <= 0: an idle slot) gets zeros;
+ * positions beyond the table hold no keys.  Keys and values outside the
+ * range, in the same page too, are never used whatever they hold.  Results
+ * do not change from call to call. */
+int xe_paged_attn_dev(xe_ctx *ctx, const xe_paged_kv *kv, const float *q_dev,
+                      uint64_t ldq, const int32_t *lens_dev, int hq,
+                      float scale, int window, float *out_dev, uint64_t ldo);
+
+/* ---- int8 linear with a scale a row ---- */
+enum xe_act {
+  XE_ACT_NONE = 0,
+  XE_ACT_RELU = 1,
+  XE_ACT_GELU = 2,  /* z (1 + erf(z / sqrt 2)) / 2 */
+  XE_ACT_SILU = 3,  /* z / (1 + exp(-z)) */
+  XE_ACT_GEGLU = 4  /* weight rows in pairs (2r gate, 2r + 1 up): y[r] =
+                       gelu_tanh(z[2r]) * z[2r + 1], m / 2 outputs */
+};
+/* Rows of xe_w8a8_rows_dev: device memory, fp32, dense. */
+typedef struct xe_w8a8_rows {
+  const float *x;      /* [batch, k] */
+  const float *add;    /* [batch, k] added to x (a sublayer's output), or null */
+  const float *post_w; /* [k]: add goes through RMSNorm (1 + w) first, with
+                          post_eps (Gemma's post norms), or null */
+  float *sum;          /* [batch, k] receives x + add, or null; may be x or add */
+  const float *res;    /* [batch, outputs] added after the activation, or null */
+  float *y;            /* [batch, outputs]; may be res */
+  int batch;           /* 1..512 */
+  int act;             /* enum xe_act */
+  float post_eps;      /* read with post_w alone */
+} xe_w8a8_rows;
+/* W8A8 linear over an XE_I8 weight: t = x + add, h = t through the weight's
+ * pre-norm, int8 codes q = round(h / s) (half away from zero) with a scale
+ * s = max|h| / 127 a row (1 for a row of zeros), and
+ * y = act(((q . w) * s) * ws[c] + bias[c]) + res, the product exact and each
+ * step in fp32 (infinite where it leaves fp32's range).  Unlike xe_w8a8_linear, whose
+ * one scale spans all rows (ctx2.rs:1352-1377), a row's result does not depend
+ * on the rows beside it.  A row with a NaN or an infinity in h gives NaN.
+ * K up to 32768. */
+int xe_w8a8_rows_dev(xe_ctx *ctx, const xe_weight *w, const xe_w8a8_rows *rows);
+
 /* Wait for the ctx stream; returns 0 or -1. */
 int xe_ctx_synchronize(xe_ctx *ctx);
 

@@ -12,6 +12,7 @@
 #include <mutex>
 
 #include "common.h"
+#include "paged.h"
 #include "quant.h"
 
 namespace xe {
@@ -111,6 +112,17 @@ char *xe_ctx::ensure_w8a8(size_t aq_bytes) {
     w8a8_ws_size = n;
   }
   return w8a8_ws;
+}
+
+char *xe_ctx::ensure_rows(size_t n) {
+  if (n > rows_ws_size) {
+    if (rows_ws) XE_HIP(hipFree(rows_ws));
+    rows_ws = nullptr;
+    rows_ws_size = 0;
+    XE_HIP(hipMalloc(&rows_ws, n));
+    rows_ws_size = n;
+  }
+  return rows_ws;
 }
 
 void xe_ctx::ensure_gemm(size_t xn_floats) {
@@ -267,6 +279,8 @@ void launch_linear(xe_ctx *ctx, const xe_weight *w, const void *x, int x_dtype, 
   ctx->dispatches++;
 }
 
+constexpr int kMaxPagedHeads = 1024;
+
 // int8 x int8 -> i32 with an output stage: the sdot4 GEMV up to 8 rows, the
 // int8 MFMA GEMM beyond.
 void launch_i8act(xe_ctx *ctx, const xe_weight *w, const int8_t *xq_dev, int batch, const W8a8Epi &e,
@@ -333,6 +347,34 @@ int run_gemv_host(xe_ctx *ctx, const xe_weight *w, const void *x, int x_dtype, i
 }
 
 }  // namespace
+
+PagedView xe::paged_view(const xe_paged_kv *kv) {
+  XE_REQUIRE(kv->k && kv->v && kv->table, "paged cache: null keys, values or table");
+  XE_REQUIRE(((reinterpret_cast<uintptr_t>(kv->k) | reinterpret_cast<uintptr_t>(kv->v)) & 15) == 0,
+             "paged cache: keys and values must be 16-byte aligned");
+  XE_REQUIRE(kv->hd == 64 || kv->hd == 128 || kv->hd == 256, "paged cache: hd must be 64, 128 or 256");
+  XE_REQUIRE(kv->page_size >= 16 && kv->page_size <= 1024 && (kv->page_size & (kv->page_size - 1)) == 0,
+             "paged cache: page_size must be a power of two, 16..1024");
+  XE_REQUIRE(kv->hkv >= 1 && kv->hkv <= kMaxPagedHeads && kv->n_pages >= 1, "paged cache: bad heads or pages");
+  XE_REQUIRE(kv->batch >= 1 && kv->batch <= 4096, "paged cache: batch must be 1..4096");
+  XE_REQUIRE(kv->max_pages >= 1 && static_cast<int64_t>(kv->max_pages) * kv->page_size <= (1 << 30),
+             "paged cache: max_pages * page_size must be 1..2^30");
+  PagedView v;
+  v.k = kv->k;
+  v.v = kv->v;
+  v.table = kv->table;
+  const uint64_t dense = static_cast<uint64_t>(kv->hkv) * kv->page_size * kv->hd;
+  v.page_stride = kv->page_stride ? kv->page_stride : dense;
+  XE_REQUIRE(v.page_stride >= dense && v.page_stride % 8 == 0 && v.page_stride <= (uint64_t(1) << 40),
+             "paged cache: page_stride below a page or no multiple of 8");
+  v.n_pages = kv->n_pages;
+  while ((1 << v.page_shift) < kv->page_size) v.page_shift++;
+  v.hkv = kv->hkv;
+  v.hd = kv->hd;
+  v.batch = kv->batch;
+  v.max_pages = kv->max_pages;
+  return v;
+}
 
 // ===========================================================================
 // extern "C"
@@ -477,6 +519,7 @@ void xe_ctx_destroy(xe_ctx *ctx) {
     if (ctx->gemm_cnt) (void)hipFree(ctx->gemm_cnt);
     if (ctx->gemm_xn) (void)hipFree(ctx->gemm_xn);
     if (ctx->w8a8_ws) (void)hipFree(ctx->w8a8_ws);
+    if (ctx->rows_ws) (void)hipFree(ctx->rows_ws);
     delete ctx;
     return 0;
   }, -1);
@@ -1003,6 +1046,98 @@ int xe_attn_decode(xe_ctx *ctx, const float *q, const uint16_t *kc, const uint16
     attn_impl(ctx, dq, dk, dv, dl, batch, hq, hkv, hd, max_ctx, scale, dout);
     XE_HIP(hipMemcpyAsync(out, dout, qn * 4, hipMemcpyDeviceToHost, s));
     XE_HIP(hipStreamSynchronize(s));
+    return 0;
+  }, -1);
+}
+
+// ---- paged KV cache, int8 linears with a scale a row ----------------------
+
+int xe_paged_append_dev(xe_ctx *ctx, const xe_paged_kv *kv, const xe_paged_rows *rows) {
+  return guard([&]() -> int {
+    XE_REQUIRE(kv && rows, "null argument");
+    const PagedView v = paged_view(kv);
+    xe_paged_rows r = *rows;
+    XE_REQUIRE(r.k && r.v && r.pos, "paged append: null keys, values or positions");
+    XE_REQUIRE(r.n_rows >= 1 && r.n_rows <= (1 << 30), "paged append: n_rows must be 1..2^30");
+    XE_REQUIRE(r.start || r.n_rows == v.batch, "paged append: without start there is one row a stream");
+    const uint64_t kvw = static_cast<uint64_t>(v.hkv) * v.hd, most = uint64_t(1) << 30;
+    XE_REQUIRE(r.ldkv >= kvw && r.ldkv <= most, "paged append: ldkv below hkv * hd");
+    if (r.q) {
+      XE_REQUIRE(r.hq >= 1 && r.hq <= kMaxPagedHeads, "paged append: hq must be 1..1024");
+      const uint64_t qw = static_cast<uint64_t>(r.hq) * v.hd;
+      XE_REQUIRE(r.q_out, "paged append: q without q_out");
+      XE_REQUIRE(r.ldq >= qw && r.ldq <= most && r.ldqo >= qw && r.ldqo <= most, "paged append: ldq or ldqo below hq * hd");
+      XE_REQUIRE(r.q_out != r.q || r.ldqo == r.ldq, "paged append: q_out over q needs its row stride");
+    } else {
+      XE_REQUIRE(!r.q_out && !r.q_norm_w, "paged append: q_out or q_norm_w without q");
+      r.hq = 0;
+    }
+    XE_REQUIRE(!r.rope_cos == !r.rope_sin, "paged append: one of rope_cos and rope_sin");
+    XE_REQUIRE(!r.rope_cos || r.rope_len >= 1, "paged append: rope_len must be positive");
+    XE_REQUIRE((!r.q_norm_w && !r.k_norm_w) || r.eps >= 0.f, "paged append: eps must not be negative");
+    XE_REQUIRE(ctx, "null ctx");
+    DeviceGuard dg(ctx->dev->ordinal);
+    launch_paged_append(v, r, ctx->dev->stream);
+    ctx->dispatches++;
+    return 0;
+  }, -1);
+}
+
+int xe_paged_attn_dev(xe_ctx *ctx, const xe_paged_kv *kv, const float *q_dev, uint64_t ldq, const int32_t *lens_dev,
+                      int hq, float scale, int window, float *out_dev, uint64_t ldo) {
+  return guard([&]() -> int {
+    XE_REQUIRE(kv && q_dev && lens_dev && out_dev, "null argument");
+    PagedAttn a;
+    a.kv = paged_view(kv);
+    XE_REQUIRE(hq >= 1 && hq <= kMaxPagedHeads && hq % a.kv.hkv == 0, "paged attention: hq must be a multiple of hkv, 1..1024");
+    const uint64_t qw = static_cast<uint64_t>(hq) * a.kv.hd, most = uint64_t(1) << 30;
+    a.q = q_dev;
+    a.ldq = ldq ? ldq : qw;
+    a.lens = lens_dev;
+    a.hq = hq;
+    a.scale = scale;
+    a.window = window;
+    a.out = out_dev;
+    a.ldo = ldo ? ldo : qw;
+    XE_REQUIRE(a.ldq >= qw && a.ldq <= most && a.ldo >= qw && a.ldo <= most, "paged attention: ldq or ldo below hq * hd");
+    XE_REQUIRE(window >= 0, "paged attention: window must not be negative");
+    XE_REQUIRE(std::isfinite(scale), "paged attention: scale must be finite");
+    XE_REQUIRE(ctx, "null ctx");
+    DeviceGuard dg(ctx->dev->ordinal);
+    launch_paged_attn(a, ctx->dev->stream);
+    ctx->dispatches++;
+    return 0;
+  }, -1);
+}
+
+int xe_w8a8_rows_dev(xe_ctx *ctx, const xe_weight *w, const xe_w8a8_rows *rows) {
+  return guard([&]() -> int {
+    XE_REQUIRE(rows && rows->x && rows->y, "null argument");
+    XE_REQUIRE(rows->batch >= 1 && rows->batch <= kMaxOpBatch, "batch must be 1..512");
+    XE_REQUIRE(rows->act >= XE_ACT_NONE && rows->act <= XE_ACT_GEGLU, "unknown activation");
+    XE_REQUIRE(!rows->post_w || (rows->add && rows->post_eps >= 0.f), "post_w needs add and an eps of zero or more");
+    XE_REQUIRE(ctx && w, "null ctx or weight");
+    XE_REQUIRE(w->wdtype == XE_I8, "xe_w8a8_rows needs an XE_I8 weight");
+    XE_REQUIRE(rows->act != XE_ACT_GEGLU || w->m % 2 == 0, "XE_ACT_GEGLU needs weight rows in pairs");
+    XE_REQUIRE(w->k <= 32768, "xe_w8a8_rows: K beyond 32768");
+    XE_REQUIRE(static_cast<size_t>(w->m) * w->k < (size_t(1) << 31), "xe_w8a8_rows: weight above 2 GB");
+    DeviceGuard dg(ctx->dev->ordinal);
+    RowsQ8 r;
+    r.w = static_cast<const int8_t *>(w->w);
+    r.ws = w->scale;
+    r.bias = w->bias;
+    r.m = w->m;
+    r.k = w->k;
+    r.norm = w->norm;
+    r.gamma = w->gamma;
+    r.beta = w->beta;
+    r.eps = w->eps;
+    r.a = *rows;
+    char *ws = ctx->ensure_rows(2048 + static_cast<size_t>(rows->batch) * w->k);
+    r.scales = reinterpret_cast<float *>(ws);
+    r.codes = reinterpret_cast<int8_t *>(ws + 2048);
+    launch_rows_q8(r, ctx->dev->stream);
+    ctx->dispatches += 2;
     return 0;
   }, -1);
 }

@@ -101,6 +101,10 @@ struct xe_ctx {
   char *w8a8_ws = nullptr;
   size_t w8a8_ws_size = 0;
   char *ensure_w8a8(size_t aq_bytes);
+  // int8 linears with a scale a row: the scales and the codes
+  char *rows_ws = nullptr;
+  size_t rows_ws_size = 0;
+  char *ensure_rows(size_t n);
   void *ensure_scratch(size_t n);
   void ensure_gemm(size_t xn_floats);
   void *ensure_pinned(size_t n);

@@ -29,6 +29,7 @@ XE_EPI_NONE, XE_EPI_BIAS, XE_EPI_SILU_BIAS = 0, 1, 2
 XE_Q8_LIN, XE_Q8_ELF = 0, 1
 XE_NORM_NONE, XE_NORM_LN, XE_NORM_RMS, XE_NORM_RMS1P = 0, 1, 2, 3
 XE_LAYOUT_MK, XE_LAYOUT_KN = 0, 1
+XE_ACT_NONE, XE_ACT_RELU, XE_ACT_GELU, XE_ACT_SILU, XE_ACT_GEGLU = 0, 1, 2, 3, 4
 XE_OPT, XE_WHISPER, XE_GEMMA3 = 0, 1, 2
 EXECUTORS = {0: "graph", 2: "eager", 3: "ll"}
 LINEAR_KERNELS = ("gemv", "gemm", "planes", "planes_big")  # enum xe_linear_kernel
@@ -54,6 +55,7 @@ EXPORTS = [
     "xe_decoder_generate_until",
     "xe_decoder_feed", "xe_decoder_decode", "xe_decoder_profile_step", "xe_decoder_executor",
     "xe_decoder_prompt_pass", "xe_linear_path", "xe_attn_splits",
+    "xe_paged_append_dev", "xe_paged_attn_dev", "xe_w8a8_rows_dev",
     "xe_model_tensor_shape", "xe_decoder_config", "xe_decoder_load_safetensors", "xe_safetensors_plan",
     "xe_ctx_record", "xe_run_query", "xe_run_wait", "xe_run_free", "xe_resident_open", "xe_resident_close",
     "xe_resident_write", "xe_resident_dispatch", "xe_resident_dispatch_start", "xe_resident_read",
@@ -79,6 +81,39 @@ class ModelConfig(C.Structure):
 
     def as_dict(self):
         return {name: getattr(self, name) for name, _ in self._fields_}
+
+
+class PagedKV(C.Structure):
+    """xe_paged_kv: a KV cache in pages over device buffers (anything with
+    .ptr; they must outlive it).  k, v bf16 [n_pages, hkv, page_size, hd],
+    table int32 [batch, max_pages]."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("table", C.c_void_p), ("page_stride", C.c_uint64)] + \
+               [(n, C.c_int) for n in ("n_pages", "hkv", "page_size", "hd", "batch", "max_pages")]
+
+    def __init__(self, k, v, table, n_pages, hkv, page_size, hd, batch, max_pages, page_stride=0):
+        super().__init__(k.ptr, v.ptr, table.ptr, page_stride, n_pages, hkv, page_size, hd, batch, max_pages)
+
+
+class PagedRows(C.Structure):
+    """xe_paged_rows: device addresses of the rows that paged_append_dev takes."""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("ldq", C.c_uint64), ("ldkv", C.c_uint64),
+                ("q_out", C.c_void_p), ("ldqo", C.c_uint64), ("pos", C.c_void_p), ("start", C.c_void_p),
+                ("q_norm_w", C.c_void_p), ("k_norm_w", C.c_void_p), ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p),
+                ("eps", C.c_float), ("rope_len", C.c_int), ("n_rows", C.c_int), ("hq", C.c_int)]
+
+    def __init__(self, n_rows, hq, q=None, k=None, v=None, ldq=0, ldkv=0, q_out=None, ldqo=0, pos=None, start=None,
+                 q_norm=None, k_norm=None, eps=1e-6, cos=None, sin=None, rope_len=0):
+        super().__init__(q, k, v, ldq, ldkv, q_out, ldqo, pos, start, q_norm, k_norm, cos, sin, eps, rope_len, n_rows, hq)
+
+
+class W8a8Rows(C.Structure):
+    """xe_w8a8_rows: device addresses of the rows that w8a8_rows_dev takes."""
+    _fields_ = [("x", C.c_void_p), ("add", C.c_void_p), ("post_w", C.c_void_p), ("sum", C.c_void_p),
+                ("res", C.c_void_p), ("y", C.c_void_p), ("batch", C.c_int), ("act", C.c_int),
+                ("post_eps", C.c_float)]
+
+    def __init__(self, batch, x, y, act=XE_ACT_NONE, add=None, post_w=None, sum=None, res=None, post_eps=1e-6):
+        super().__init__(x, add, post_w, sum, res, y, batch, act, post_eps)
 
 
 def _cfg(**kw):
@@ -181,6 +216,9 @@ def lib():
         "xe_decoder_prompt_pass": (i, [vp, i, i]),
         "xe_attn_splits": (i, [vp, i, i, i, i, i, C.POINTER(i)]),
         "xe_linear_path": (i, [i, i, i, i, i, i, C.POINTER(i)]),
+        "xe_paged_append_dev": (i, [vp, C.POINTER(PagedKV), C.POINTER(PagedRows)]),
+        "xe_paged_attn_dev": (i, [vp, C.POINTER(PagedKV), vp, u64, vp, i, f, i, vp, u64]),
+        "xe_w8a8_rows_dev": (i, [vp, vp, C.POINTER(W8a8Rows)]),
         "xe_ctx_record": (vp, [vp]),
         "xe_run_query": (i, [vp]),
         "xe_run_wait": (i, [vp]),
@@ -506,6 +544,21 @@ class CtxDecode:
     def attn_dev(self, q_buf, k_buf, v_buf, lens_buf, b, hq, hkv, hd, max_ctx, scale, out_buf):
         _check(lib().xe_attn_decode_dev(self.h, q_buf.ptr, k_buf.ptr, v_buf.ptr, lens_buf.ptr, b,
                                         hq, hkv, hd, max_ctx, scale, out_buf.ptr))
+
+    # -- paged KV cache (device buffers, asynchronous) --
+    def paged_append_dev(self, kv, rows):
+        """New tokens' rows into their streams' pages; queries normalised and
+        rotated into rows.q_out (xe_paged_append_dev)."""
+        _check(lib().xe_paged_append_dev(self.h, kv, rows))
+
+    def paged_attn_dev(self, kv, q_buf, lens_buf, hq, scale, out_buf, window=0, ldq=0, ldo=0):
+        """One query token a stream over its pages (xe_paged_attn_dev)."""
+        _check(lib().xe_paged_attn_dev(self.h, kv, q_buf.ptr, ldq, lens_buf.ptr, hq, scale, window, out_buf.ptr, ldo))
+
+    def w8a8_rows_dev(self, weight, rows):
+        """int8 linear with a scale a row: residual addition and norm before
+        it, bias, activation and residual after it (xe_w8a8_rows_dev)."""
+        _check(lib().xe_w8a8_rows_dev(self.h, weight.h, rows))
 
 
 class Run:
