@@ -72,6 +72,56 @@ int main() {
     subprocess.check_call([exe], timeout=60)
 
 
+def test_shares(tmp_path):
+    """Every granule belongs to exactly one workgroup, each workgroup's partials
+    to places of their own, and a unit's partials are found where they lie."""
+    if shutil.which("g++") is None:
+        pytest.skip("no g++")
+    src = tmp_path / "s.cpp"
+    src.write_text(r'''
+#include "paged_index.h"
+#include <cassert>
+#include <random>
+#include <set>
+#include <vector>
+using namespace xe::paged;
+int main() {
+  std::mt19937 rng(3);
+  auto pick = [&](int n) { return (int)(rng() % n); };
+  assert(granules(0, 0, 256) == 0 && granules(5, 6, 256) == 1 && granules(0, 256, 256) == 1 && granules(0, 257, 256) == 2);
+  assert(granules(15, 256, 256) == 1 && granules(17, 272, 256) == 1 && granules(17, 273, 256) == 2);
+  for (int round = 0; round < 3000; round++) {
+    const int units = 1 + pick(40), most = 1 << pick(10);
+    std::vector<unsigned> n(units);
+    unsigned total = 0;
+    for (auto &x : n) total += x = pick(3) ? 1 + pick(most) : 1;
+    const unsigned nwg = pick(2) ? 512 : 1 + pick(512), least = pick(2) ? 1 : 1 + pick(9);
+    const unsigned per = share_of(total, nwg, least);
+    assert(per >= 1 && (unsigned long long)per * nwg >= total);
+    std::set<unsigned> places;
+    unsigned u0 = 0, covered = 0;
+    for (int u = 0; u < units; u++) {
+      const unsigned u1 = u0 + n[u], w0 = first_wg(u0, per), cnt = wg_count(u0, u1, per);
+      assert(cnt >= 1 && w0 + cnt <= nwg);
+      for (unsigned wg = w0; wg < w0 + cnt; wg++) {
+        const unsigned a = wg * per > u0 ? wg * per : u0, z = (wg + 1) * per < u1 ? (wg + 1) * per : u1;
+        assert(a < z);
+        covered += z - a;
+        const unsigned slot = slot_of(u0, per, wg);
+        assert(slot < 2 * nwg);
+        if (cnt > 1) assert(places.insert(slot).second);
+      }
+      u0 = u1;
+    }
+    assert(covered == total);
+  }
+}
+''')
+    exe = str(tmp_path / "s")
+    subprocess.check_call(["g++", "-O1", "-std=c++17", "-fsanitize=undefined,address", "-I" + CSRC, str(src), "-o", exe])
+    subprocess.check_call([exe], timeout=60)
+
+
 def fails(xe, call, *args):
     assert call(None, *args) == -1
     return xe.last_error()

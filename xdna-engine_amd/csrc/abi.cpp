@@ -125,6 +125,18 @@ char *xe_ctx::ensure_rows(size_t n) {
   return rows_ws;
 }
 
+void xe_ctx::ensure_paged() {
+  if (!paged_work) XE_HIP(hipMalloc(&paged_work, paged_work_floats() * sizeof(float)));
+  if (!paged_cnt) {
+    unsigned *cnt = nullptr;
+    XE_HIP(hipMalloc(&cnt, paged_cnt_words() * sizeof(unsigned)));
+    const hipError_t e = hipMemsetAsync(cnt, 0, paged_cnt_words() * sizeof(unsigned), dev->stream);
+    if (e != hipSuccess) (void)hipFree(cnt);
+    XE_HIP(e);
+    paged_cnt = cnt;
+  }
+}
+
 void xe_ctx::ensure_gemm(size_t xn_floats) {
   if (!gemm_ws) {
     XE_HIP(hipMalloc(&gemm_ws, gemm_op_ws_floats() * sizeof(float)));
@@ -520,6 +532,8 @@ void xe_ctx_destroy(xe_ctx *ctx) {
     if (ctx->gemm_xn) (void)hipFree(ctx->gemm_xn);
     if (ctx->w8a8_ws) (void)hipFree(ctx->w8a8_ws);
     if (ctx->rows_ws) (void)hipFree(ctx->rows_ws);
+    if (ctx->paged_work) (void)hipFree(ctx->paged_work);
+    if (ctx->paged_cnt) (void)hipFree(ctx->paged_cnt);
     delete ctx;
     return 0;
   }, -1);
@@ -1104,7 +1118,8 @@ int xe_paged_attn_dev(xe_ctx *ctx, const xe_paged_kv *kv, const float *q_dev, ui
     XE_REQUIRE(std::isfinite(scale), "paged attention: scale must be finite");
     XE_REQUIRE(ctx, "null ctx");
     DeviceGuard dg(ctx->dev->ordinal);
-    launch_paged_attn(a, ctx->dev->stream);
+    ctx->ensure_paged();
+    launch_paged_attn(a, ctx->paged_work, ctx->paged_cnt, ctx->dev->stream);
     ctx->dispatches++;
     return 0;
   }, -1);

@@ -105,6 +105,11 @@ struct xe_ctx {
   char *rows_ws = nullptr;
   size_t rows_ws_size = 0;
   char *ensure_rows(size_t n);
+  // attention over pages: partials and arrival counters (zeroed once,
+  // self-resetting), allocated by the first call
+  float *paged_work = nullptr;
+  unsigned *paged_cnt = nullptr;
+  void ensure_paged();
   void *ensure_scratch(size_t n);
   void ensure_gemm(size_t xn_floats);
   void *ensure_pinned(size_t n);

@@ -29,7 +29,12 @@ struct PagedAttn {
   float *out = nullptr;
   size_t ldo = 0;
 };
-void launch_paged_attn(const PagedAttn &a, hipStream_t s);
+// work / cnt: partials of units that several workgroups share
+// (paged_work_floats()) and arrival counters (paged_cnt_words(), zeroed once;
+// they re-arm).
+void launch_paged_attn(const PagedAttn &a, float *work, unsigned *cnt, hipStream_t s);
+size_t paged_work_floats();
+size_t paged_cnt_words();
 
 // y = act((q . w) s ws + bias) + res over the int8 codes q of norm(x + add)
 // and their row scales s; codes / scales: workspace, batch * k bytes and batch

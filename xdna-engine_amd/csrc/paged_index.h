@@ -36,5 +36,28 @@ XE_HD void key_range(int len, int window, int capacity, int &lo, int &hi) {
   if (hi < lo) hi = lo;
 }
 
+// Attention's work is counted in granules of kg keys (kg a power of two), the
+// first of a stream at the last multiple of 16 at or before its first key.
+XE_HD unsigned granules(int lo, int hi, int kg) {
+  return hi > lo ? static_cast<unsigned>((hi - (lo & ~15) + (kg - 1)) / kg) : 0u;
+}
+
+// The granules of all units -- unit (stream, block of query heads), stream by
+// stream -- in a row, [0, total), are shared out in equal ranges: workgroup i
+// takes [i * per, (i + 1) * per).
+XE_HD unsigned share_of(unsigned total, unsigned workgroups, unsigned least) {
+  const unsigned per = (total + workgroups - 1) / workgroups;
+  return per < least ? least : per;
+}
+
+// Workgroups that the unit of granules [u0, u1) is spread over: first_wg(u0)
+// and the ones behind it.
+XE_HD unsigned first_wg(unsigned u0, unsigned per) { return u0 / per; }
+XE_HD unsigned wg_count(unsigned u0, unsigned u1, unsigned per) { return (u1 - 1) / per - u0 / per + 1; }
+
+// Place of workgroup wg's partial of that unit: a workgroup has at most one
+// unit that began before it and one that it begins and does not end.
+XE_HD unsigned slot_of(unsigned u0, unsigned per, unsigned wg) { return 2 * wg + (u0 >= wg * per ? 1u : 0u); }
+
 }  // namespace paged
 }  // namespace xe
