@@ -95,13 +95,13 @@ int main() {
     std::vector<unsigned> n(units);
     unsigned total = 0;
     for (auto &x : n) total += x = pick(3) ? 1 + pick(most) : 1;
-    const unsigned nwg = pick(2) ? 512 : 1 + pick(512), least = pick(2) ? 1 : 1 + pick(9);
-    const unsigned per = share_of(total, nwg, least);
+    const unsigned nwg = pick(2) ? 256 : 1 + pick(512), per = share_of(total, nwg);
+    const Div by = div_by(per);
     assert(per >= 1 && (unsigned long long)per * nwg >= total);
     std::set<unsigned> places;
     unsigned u0 = 0, covered = 0;
     for (int u = 0; u < units; u++) {
-      const unsigned u1 = u0 + n[u], w0 = first_wg(u0, per), cnt = wg_count(u0, u1, per);
+      const unsigned u1 = u0 + n[u], w0 = quot(u0, by), cnt = quot(u1 - 1, by) - w0 + 1;
       assert(cnt >= 1 && w0 + cnt <= nwg);
       for (unsigned wg = w0; wg < w0 + cnt; wg++) {
         const unsigned a = wg * per > u0 ? wg * per : u0, z = (wg + 1) * per < u1 ? (wg + 1) * per : u1;
@@ -114,6 +114,26 @@ int main() {
       u0 = u1;
     }
     assert(covered == total);
+    for (int u = 0; u < units; u++) {  // whole workgroups
+      const unsigned wgs = quot_up(n[u], by);
+      unsigned upto = 0, most = 0, least = ~0u;
+      for (unsigned i = 0; i < wgs; i++) {
+        unsigned t0, t1;
+        part_of(n[u], wgs, i, t0, t1);
+        assert(t0 == upto && t1 > t0 && t1 - t0 <= per);
+        upto = t1;
+        most = t1 - t0 > most ? t1 - t0 : most;
+        least = t1 - t0 < least ? t1 - t0 : least;
+      }
+      assert(upto == n[u] && most - least <= 1);
+    }
+  }
+  for (int round = 0; round < 300000; round++) {
+    unsigned a = rng(), d = rng() >> (rng() % 32);
+    if (round % 7 == 0) a = ~0u - pick(3);
+    if (round % 5 == 0) a = (a / (d ? d : 1)) * (d ? d : 1) - pick(2);
+    if (d == 0) d = 1;
+    assert(quot(a, div_by(d)) == a / d && quot_up(a, div_by(d)) == a / d + (a % d != 0));
   }
 }
 ''')

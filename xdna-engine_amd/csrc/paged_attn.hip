@@ -42,17 +42,26 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
-#ifndef XE_PA_EU
-#define XE_PA_EU 2
-#endif
-#ifndef XE_PA_L
-#define XE_PA_L 1
-#endif
 constexpr int kTile = 16;    // keys a wave takes at a time, and a granule
 constexpr int kRows = 16;    // query heads a unit at most
-constexpr int kMaxWg = 1024;
+constexpr int kMaxWg = 512;
 constexpr int kGroup = 16;   // partials merged at once
 constexpr int kMaxHd = 256;
+// Fewer units than this: workgroups of eight waves, one a CU, whole ones a
+// unit, so that a workgroup has one unit's chain of loads before it; else of
+// four, two a CU, in equal shares.  us with eight / four waves: 32768 keys of
+// one stream (4 x 256) 19.7 / 23.6, 60000 keys (7 x 128) 16.7 / 21.1, 8 mixed
+// streams to 3000 keys (8 / 2 x 128, 16 units) 10.9 / 10.8, 64 streams to 4096
+// (4 x 256, 64 units) 50.3 / 46.9, 192 mixed to 5000 (6 / 2 x 64) 59.6 / 54.3.
+// Nontemporal loads where the keys are many, us plain / nontemporal: 150 mixed
+// streams to 8192 keys (16 / 2 x 128) 113 / 103, 48 to 8192 (12 x 64) 159 / 145;
+// 32768 keys of one stream 19.7 / 20.3.
+constexpr int kManyUnits = 64;
+// Whole workgroups a unit: units of up to kAlone tiles in one workgroup (28
+// tiles, 12 units of hd 64: 7.7 us, in two workgroups each 8.9), up to kMore
+// tiles a workgroup where a second level of merges is avoided with them (188
+// tiles of hd 256: 14.9 us, 15.9 with a tile a workgroup).
+constexpr unsigned kAlone = 32, kMore = 24;
 
 __device__ __forceinline__ uint32_t hi16(uint32_t lo, uint32_t hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
 __device__ __forceinline__ uint32_t lo16(uint32_t lo, uint32_t hi) { return __builtin_amdgcn_perm(hi, lo, 0x05040100u); }
@@ -85,6 +94,32 @@ __device__ __forceinline__ float rows_sum(float v) {
   return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
 
+// op over the wave, in every lane, and the sum of the lanes up to this one:
+// by DPP and lane swaps, without the LDS crossbar.
+template <typename Op>
+__device__ __forceinline__ unsigned wave_all(unsigned v, Op op) {
+  v = op(v, static_cast<unsigned>(gdev::dpp_get_i<gdev::kDppXor1>(static_cast<int>(v))));
+  v = op(v, static_cast<unsigned>(gdev::dpp_get_i<gdev::kDppXor2>(static_cast<int>(v))));
+  v = op(v, static_cast<unsigned>(gdev::dpp_get_i<gdev::kDppHalfMirror>(static_cast<int>(v))));
+  v = op(v, static_cast<unsigned>(gdev::dpp_get_i<gdev::kDppMirror>(static_cast<int>(v))));
+  const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = op(r[0], r[1]);
+  const auto s = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return __builtin_amdgcn_readfirstlane(op(s[0], s[1]));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned add_from(unsigned v) {
+  return v + static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false));
+}
+__device__ __forceinline__ unsigned wave_scan(unsigned v) {
+  v = add_from<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8: within 16 lanes
+  v = add_from<0x112, 0xF>(v);
+  v = add_from<0x114, 0xF>(v);
+  v = add_from<0x118, 0xF>(v);
+  v = add_from<0x142, 0xA>(v);  // lane 15 to the next row
+  return add_from<0x143, 0xC>(v);  // lane 31 to the upper half
+}
+
 struct Params {
   PagedAttn a;
   float *work;
@@ -93,13 +128,13 @@ struct Params {
   int blocks;           // units of a kv head
   int rows;             // query heads a unit holds room for: min(group, 16)
   unsigned slot_floats; // a partial: O [rows][hd], m [rows], l [rows]
-  unsigned least;       // granules a workgroup takes at least
 };
 
 constexpr size_t slot_floats_of(int hd, int rows) { return (static_cast<size_t>(rows) * (hd + 2) + 3) & ~size_t(3); }
+constexpr int kPad = 4;  // floats between the rows that waves write beside each other
 // bytes of the area that holds the queries of a unit, then what its waves found
 constexpr size_t area_bytes(int hd, int rows, int kw) {
-  const size_t q = static_cast<size_t>(3) * kRows * hd * 2, meet = (static_cast<size_t>(kw) * rows * hd + 2 * kw * kRows) * 4;
+  const size_t q = static_cast<size_t>(3) * kRows * hd * 2, meet = (static_cast<size_t>(kw) * rows * (hd + kPad) + 2 * kw * kRows) * 4;
   return q > meet ? q : meet;
 }
 
@@ -109,9 +144,17 @@ __device__ __forceinline__ void put4(float *base, unsigned idx, const f32x4 &v) 
                                          gdev::kCoherentSc1);
 }
 
+template <bool NT, typename P>
+__device__ __forceinline__ auto load(P p) {
+  if constexpr (NT) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+
 template <int HD, int KW>
-__global__ __launch_bounds__(64 * KW, KW == 8 ? 2 : XE_PA_EU) void paged_attn_kernel(Params p) {
+__global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(Params p) {
   constexpr int T = 64 * KW;
+  constexpr bool kWhole = KW == 8;          // whole workgroups a unit; else equal shares of all keys
+  constexpr bool kStream = KW == 4;         // keys and values by nontemporal loads
   constexpr int S = HD / 32;                // 32-dimension steps of a score
   constexpr int VB = HD >= 128 ? 8 : 4;     // dimensions of a value a lane loads at once
   constexpr int HV = HD / (16 * VB);        // loads of a value row
@@ -123,38 +166,31 @@ __global__ __launch_bounds__(64 * KW, KW == 8 ? 2 : XE_PA_EU) void paged_attn_ke
   unsigned char *const qs = lds;                                              // [3][S][64] x 16 bytes
   float *const meet = reinterpret_cast<float *>(lds);                         // [KW][rows][HD], m and l [KW][kRows]
   int32_t *const lens = reinterpret_cast<int32_t *>(lds + area_bytes(HD, p.rows, KW));  // [batch]
+  unsigned *const count = reinterpret_cast<unsigned *>(lens + p.a.kv.batch);            // [batch] granules of a unit
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int ln = lane & 15, lg = lane >> 4;
   const PagedView &kv = p.a.kv;
   const int batch = kv.batch, H = kv.hkv * p.blocks;
   const int cap = kv.max_pages << kv.page_shift;
   const unsigned wg = blockIdx.x, nwg = gridDim.x;
 
-  // Granules of the streams: this thread's, the sum before them, all of them.
-  // Up to 64 streams every wave adds them up itself, a stream a lane.
-  const bool few = batch <= 64;
-  const int me = few ? lane : tid, each = few ? 1 : (batch + T - 1) / T;
-  auto stream_granules = [&](int b) {
-    int lo, hi;
-    paged::key_range(lens[b], p.a.window, cap, lo, hi);
-    return paged::granules(lo, hi, kTile);
-  };
+  // Granules of the streams' units: a stream a lane of every wave (kWhole), or
+  // some a thread.
+  const int each = kWhole ? 1 : (batch + T - 1) / T;
+  const int s0 = (kWhole ? lane : tid) * each, s1 = min(s0 + each, batch);  // this thread's streams
   unsigned mine = 0;
-  for (int i = 0; i < each; i++) {
-    const int b = me * each + i;
-    if (b >= batch) break;
-    lens[b] = p.a.lens[b];
-    mine += stream_granules(b) * H;
+  for (int b = s0; b < s1; b++) {
+    const int len = p.a.lens[b];
+    int lo, hi;
+    paged::key_range(len, p.a.window, cap, lo, hi);
+    const unsigned n = paged::granules(lo, hi, kTile);
+    lens[b] = len;
+    count[b] = n;
+    mine += n;
   }
-  unsigned incl = mine;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const unsigned o = __shfl_up(incl, off, 64);
-    if (lane >= off) incl += o;
-  }
-  unsigned before = incl - mine, total = __builtin_amdgcn_readlane(incl, 63);
-  if (!few) {
+  const unsigned incl = wave_scan(mine * H);
+  unsigned before = incl - mine * H, total = __builtin_amdgcn_readlane(incl, 63);
+  if constexpr (!kWhole) {
     if (lane == 63) scan[wave] = incl;
     __syncthreads();
     total = 0;
@@ -163,32 +199,46 @@ __global__ __launch_bounds__(64 * KW, KW == 8 ? 2 : XE_PA_EU) void paged_attn_ke
       before += w < wave ? scan[w] : 0u;
       total += scan[w];
     }
+    total = __builtin_amdgcn_readfirstlane(total);
   }
   // streams without keys: zeros
   for (int b = wg; b < batch; b += nwg) {
-    if (stream_granules(b)) continue;
+    if (count[b]) continue;
     for (int i = tid; i < p.a.hq * HD; i += T) p.a.out[static_cast<size_t>(b) * p.a.ldo + i] = 0.f;
   }
   if (total == 0) return;
-  const unsigned per = paged::share_of(total, nwg, p.least);
-  unsigned g0 = wg * per;
-  const unsigned g1 = min(g0 + per, total);
-  if (g0 >= total) return;
-  int b;          // the stream of the first granule
-  unsigned base;  // its own first granule
-  const bool mine_has = g0 >= before && g0 < before + mine;
-  if (few) {
-    b = __ffsll(__ballot(mine_has)) - 1;
-    base = __builtin_amdgcn_readlane(before, b);
+
+  paged::Div per = paged::div_by(paged::share_of(total, nwg));
+  unsigned g0 = wg * per.d;
+  const unsigned g1 = min(g0 + per.d, total);
+  int b = 0;                                   // stream
+  unsigned base = 0;                           // its first granule
+  unsigned wgs = 0, part = 0, part_unit = 0;   // kWhole: the unit's workgroups, this one among them, the unit
+  if constexpr (kWhole) {
+    const unsigned units = __popcll(__ballot(mine != 0)) * H;
+    const unsigned longest = wave_all(mine, [](unsigned x, unsigned y) { return max(x, y); });
+    // the fewest granules a workgroup for which the units' workgroups suffice
+    unsigned lo = per.d, hi = nwg > units ? min(longest, paged::share_of(total, nwg - units)) : longest;
+    while (lo < hi) {
+      const unsigned mid = lo + (hi - lo) / 2;
+      if (wave_all(paged::quot_up(mine, paged::div_by(mid)) * H, [](unsigned x, unsigned y) { return x + y; }) <= nwg) hi = mid;
+      else lo = mid + 1;
+    }
+    per = paged::div_by(max(hi, paged::least_share(longest, kGroup, kAlone, kMore)));
+    const unsigned own = paged::quot_up(mine, per), upto = wave_scan(own * H);
+    const unsigned long long has = __ballot(wg < upto);
+    if (!has) return;
+    b = __ffsll(has) - 1;
+    wgs = __builtin_amdgcn_readlane(own, b);
+    const unsigned at = wg - (__builtin_amdgcn_readlane(upto, b) - wgs * H);
+    part_unit = at / wgs;
+    part = at - part_unit * wgs;
   } else {
-    if (mine_has) {
+    if (g0 >= total) return;
+    if (g0 >= before && g0 < before + mine * H) {
       unsigned sum = before;
-      int s = tid * each;
-      for (;; s++) {
-        const unsigned n = stream_granules(s) * H;
-        if (g0 < sum + n) break;
-        sum += n;
-      }
+      int s = s0;
+      for (; g0 >= sum + count[s] * H; s++) sum += count[s] * H;
       found[0] = s;
       found[1] = sum;
     }
@@ -200,21 +250,35 @@ __global__ __launch_bounds__(64 * KW, KW == 8 ? 2 : XE_PA_EU) void paged_attn_ke
   const size_t head_rows = static_cast<size_t>(1) << kv.page_shift;
   const int slot_mask = (1 << kv.page_shift) - 1;
 
-  while (g0 < g1) {
+  for (;;) {
+    int own = tid;  // opaque: addresses made from it are not kept over the units
+    asm volatile("" : "+v"(own));
+    const int ln = own & 15, lg = (own >> 4) & 3;
     int lo, hi;
     paged::key_range(__builtin_amdgcn_readfirstlane(lens[b]), p.a.window, cap, lo, hi);
-    const unsigned n = paged::granules(lo, hi, kTile);
-    if (g0 >= base + n * H) {
-      base += n * H;
-      b++;
-      continue;
+    const unsigned n = __builtin_amdgcn_readfirstlane(count[b]);
+    unsigned unit = part_unit, u0 = ~0u, ge = g1;  // partials in slots 2 i + 1
+    unsigned w0 = wg - part, nseg = wgs, t0, t1;   // the unit's workgroups, this one's granules of it
+    if constexpr (kWhole) {
+      paged::part_of(n, wgs, part, t0, t1);
+    } else {
+      if (g0 >= base + n * H) {
+        base += n * H;
+        b++;
+        continue;
+      }
+      unit = (g0 - base) / n;
+      u0 = base + unit * n;
+      ge = min(g1, u0 + n);
+      w0 = paged::quot(u0, per);
+      nseg = paged::quot(u0 + n - 1, per) - w0 + 1;
+      t0 = g0 - u0;
+      t1 = ge - u0;
     }
-    const unsigned unit = (g0 - base) / n, u0 = base + unit * n, u1 = u0 + n;
-    const unsigned ge = min(g1, u1);  // this workgroup's granules of the unit: [g0, ge)
-    const int kvh = unit / p.blocks, r0 = (unit % p.blocks) * kRows;
+    const int kvh = unit / p.blocks, r0 = (unit - kvh * p.blocks) * kRows;
     const int rows = min(p.group - r0, kRows), h0 = kvh * p.group + r0;
-    const int first = (lo & ~15) + static_cast<int>(g0 - u0) * kTile;
-    const int ntile = static_cast<int>(ge - g0);
+    const int first = (lo & ~15) + static_cast<int>(t0) * kTile;
+    const int ntile = static_cast<int>(t1 - t0);
     const int32_t *table = kv.table + static_cast<size_t>(b) * kv.max_pages;
 
     // pages of this wave's next 64 tiles, a tile a lane
@@ -240,17 +304,23 @@ __global__ __launch_bounds__(64 * KW, KW == 8 ? 2 : XE_PA_EU) void paged_attn_ke
       const int key = first + (wave + KW * i) * kTile;
       return pool + static_cast<size_t>(pg < 0 ? 0 : pg) * kv.page_stride + (kvh * head_rows + (key & slot_mask)) * HD;
     };
-    auto load_k = [&](int i) {
-      const uint16_t *r = row_of(kv.k, i);
+    // Past the last tile every lane loads the row's first values again: the
+    // number of loads in flight must not depend on a branch, or each wait would
+    // be for the keys and the values both.
+    const unsigned k_at = (ln * HD + 8 * lg) * 2, v_at = (4 * lg * HD + VB * ln) * 2;  // bytes
+    auto load_k = [&](int i, bool more) {
+      const char *r = reinterpret_cast<const char *>(row_of(kv.k, i));
+      const unsigned at = more ? k_at : 0;
 #pragma unroll
-      for (int s = 0; s < S; s++) kr[s] = *gptr(reinterpret_cast<const u32x4 *>(r + (ln * HD + 8 * lg + 32 * s)));
+      for (int s = 0; s < S; s++) kr[s] = load<kStream>(gptr(reinterpret_cast<const u32x4 *>(r + at + 64 * s)));
     };
-    auto load_v = [&](int i) {
-      const uint16_t *r = row_of(kv.v, i);
+    auto load_v = [&](int i, bool more) {
+      const char *r = reinterpret_cast<const char *>(row_of(kv.v, i));
+      const unsigned at = more ? v_at : 0;
 #pragma unroll
       for (int j = 0; j < 4; j++)
 #pragma unroll
-        for (int c = 0; c < HV; c++) vr[j][c] = *gptr(reinterpret_cast<const VReg *>(r + ((4 * lg + j) * HD + VB * ln + 16 * VB * c)));
+        for (int c = 0; c < HV; c++) vr[j][c] = load<kStream>(gptr(reinterpret_cast<const VReg *>(r + at + (j * HD + 16 * VB * c) * 2)));
     };
 
     f32x4 o[NO];
@@ -258,10 +328,8 @@ __global__ __launch_bounds__(64 * KW, KW == 8 ? 2 : XE_PA_EU) void paged_attn_ke
     for (int i = 0; i < NO; i++) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
     const int tiles = (ntile - wave + KW - 1) / KW;  // this wave's
-    if (tiles > 0) {
-      load_k(0);
-      load_v(0);
-    }
+    load_k(0, tiles > 0);
+    load_v(0, tiles > 0);
     // the queries in three parts, operand order, while the first keys load
 #pragma unroll
     for (int u = 0; u < SQ; u++) {
@@ -282,18 +350,22 @@ __global__ __launch_bounds__(64 * KW, KW == 8 ? 2 : XE_PA_EU) void paged_attn_ke
       const bool ok = __builtin_amdgcn_readlane(pages, t & 63) >= 0;
       const bool whole = ok && key0 >= lo && key0 + kTile <= hi;
       if ((t & 63) == 63) pages = pages_from(t + 1);
-      f32x4 s = {0.f, 0.f, 0.f, 0.f};
+      f32x4 sp[3];  // of each part of the queries: independent chains
+#pragma unroll
+      for (int i = 0; i < 3; i++) sp[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < S; c++)
 #pragma unroll
         for (int i = 0; i < 3; i++)
-          s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kr[c]),
-                                                      *reinterpret_cast<const bf16x8 *>(qs + ((i * S + c) * 64 + lane) * 16), s, 0, 0, 0);
-      if (t + 1 < tiles) load_k(t + 1);
+          sp[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kr[c]),
+                                                          *reinterpret_cast<const bf16x8 *>(qs + ((i * S + c) * 64 + lane) * 16),
+                                                          sp[i], 0, 0, 0);
+      const bool more = t + 1 < tiles;
+      load_k(more ? t + 1 : t, more);
       float w[4], mb = m;
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        w[i] = s[i] * sc2;
+        w[i] = (sp[0][i] + (sp[1][i] + sp[2][i])) * sc2;
         if (!whole) {
           const int key = key0 + 4 * lg + i;
           w[i] = ok && key >= lo && key < hi ? w[i] : -INFINITY;
@@ -341,12 +413,13 @@ __global__ __launch_bounds__(64 * KW, KW == 8 ? 2 : XE_PA_EU) void paged_attn_ke
                                                                       __builtin_bit_cast(s16x4, u32x2{part[i][0], part[i][1]}),
                                                                       o[c * VB + e], 0, 0, 0);
         }
-      if (t + 1 < tiles) load_v(t + 1);
+      load_v(more ? t + 1 : t, more);
     }
     l = rows_sum(l);
 
     // the waves meet
-    float *const wm = meet + static_cast<size_t>(KW) * p.rows * HD;  // [KW][kRows]
+    constexpr int RS = HD + kPad;
+    float *const wm = meet + static_cast<size_t>(KW) * p.rows * RS;  // [KW][kRows]
     float *const wl = wm + KW * kRows;
     __syncthreads();  // the queries are done with
     if (lg == 0) {
@@ -354,25 +427,23 @@ __global__ __launch_bounds__(64 * KW, KW == 8 ? 2 : XE_PA_EU) void paged_attn_ke
       wl[wave * kRows + ln] = l;
     }
     if (ln < rows) {
-      float *d = meet + (static_cast<size_t>(wave) * p.rows + ln) * HD + VB * 4 * lg;
+      float *d = meet + (wave * p.rows + ln) * RS + 4 * lg;
 #pragma unroll
-      for (int c = 0; c < HV; c++)
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-          for (int e = 0; e < VB; e += 4)  // row 4 g + i of block (c, e) is dimension 16 VB c + VB (4 g + i) + e
-            *reinterpret_cast<f32x4 *>(d + c * 16 * VB + VB * i + e) =
-                f32x4{o[c * VB + e][i], o[c * VB + e + 1][i], o[c * VB + e + 2][i], o[c * VB + e + 3][i]};
+      for (int i = 0; i < NO; i++) *reinterpret_cast<f32x4 *>(d + 16 * i) = o[i];
     }
     __syncthreads();
-    const unsigned w0 = paged::first_wg(u0, per), nseg = paged::wg_count(u0, u1, per);
+    // A head's values lie as the MFMAs left them, here and in partials: value
+    // 16 (VB c + e) + k is dimension VB (16 c + k) + e.
     float *const out = p.a.out + static_cast<size_t>(b) * p.a.ldo + static_cast<size_t>(h0) * HD;
     auto finish = [&](int i, f32x4 x, float ls) {
+      const int blk = i % HD / 16;
+      float *d = out + (i / HD * HD + VB * (16 * (blk / VB) + i % 16) + blk % VB);
+      const float inv = ls == 0.f ? 0.f : 1.0f / ls;
 #pragma unroll
-      for (int z = 0; z < 4; z++) out[i + z] = ls == 0.f ? 0.f : x[z] / ls;
+      for (int z = 0; z < 4; z++) d[VB * z] = ls == 0.f ? 0.f : x[z] * inv;
     };
-    const unsigned my_slot = paged::slot_of(u0, per, wg) * p.slot_floats;
-    for (int i = 4 * tid; i < rows * HD; i += 4 * T) {
+    const unsigned my_slot = paged::slot_of(u0, per.d, wg) * p.slot_floats;
+    for (int i = 4 * own; i < rows * HD; i += 4 * T) {
       const int r = i / HD;
       float mk[KW], mx = -INFINITY, ls = 0.f;
       f32x4 x = {0.f, 0.f, 0.f, 0.f};
@@ -381,7 +452,7 @@ __global__ __launch_bounds__(64 * KW, KW == 8 ? 2 : XE_PA_EU) void paged_attn_ke
 #pragma unroll
       for (int w = 0; w < KW; w++) {
         const float f = mk[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mk[w] - mx);
-        const f32x4 v = *reinterpret_cast<const f32x4 *>(meet + (static_cast<size_t>(w) * p.rows * HD + i));
+        const f32x4 v = *reinterpret_cast<const f32x4 *>(meet + ((w * p.rows + r) * RS + i % HD));
         ls += wl[w * kRows + r] * f;
 #pragma unroll
         for (int z = 0; z < 4; z++) x[z] += v[z] * f;
@@ -404,25 +475,25 @@ __global__ __launch_bounds__(64 * KW, KW == 8 ? 2 : XE_PA_EU) void paged_attn_ke
         const unsigned seg0 = seg / kGroup * kGroup, cnt = min(left - seg0, static_cast<unsigned>(kGroup));
         const bool final = left <= kGroup;
         unsigned *const counter = p.cnt + (step == 1 ? 0 : step == kGroup ? 2 * kMaxWg : 4 * kMaxWg) +
-                                  paged::slot_of(u0, per, w0 + seg0 * step);
+                                  paged::slot_of(u0, per.d, w0 + seg0 * step);
         const bool last = adev::last_to_arrive(counter, static_cast<int>(cnt), reinterpret_cast<int *>(found + 2));
         if (!last) break;
         if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        const unsigned dst = paged::slot_of(u0, per, w0 + seg0 * step) * p.slot_floats;
-        for (int i = 4 * tid; i < rows * HD; i += 4 * T) {
+        const unsigned dst = paged::slot_of(u0, per.d, w0 + seg0 * step) * p.slot_floats;
+        for (int i = 4 * own; i < rows * HD; i += 4 * T) {
           const int r = i / HD;
+          float mx = -INFINITY, ls = 0.f;
+          f32x4 x = {0.f, 0.f, 0.f, 0.f};
           float mk[kGroup], lk[kGroup];
           f32x4 v[kGroup];
 #pragma unroll
           for (int k = 0; k < kGroup; k++) {  // past the last one: that one again, with no weight
-            const unsigned sl = paged::slot_of(u0, per, w0 + (seg0 + min(static_cast<unsigned>(k), cnt - 1)) * step) * p.slot_floats;
+            const unsigned sl = paged::slot_of(u0, per.d, w0 + (seg0 + min(static_cast<unsigned>(k), cnt - 1)) * step) * p.slot_floats;
             mk[k] = adev::act_ld<true>(p.work, static_cast<int>(sl + p.rows * HD + r));
             lk[k] = adev::act_ld<true>(p.work, static_cast<int>(sl + p.rows * (HD + 1) + r));
             const float4 t4 = gdev::act_ld4<true>(p.work, static_cast<int>(sl + i));
             v[k] = f32x4{t4.x, t4.y, t4.z, t4.w};
           }
-          float mx = -INFINITY, ls = 0.f;
-          f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int k = 0; k < kGroup; k++) mx = fmaxf(mx, mk[k]);
 #pragma unroll
@@ -449,8 +520,9 @@ __global__ __launch_bounds__(64 * KW, KW == 8 ? 2 : XE_PA_EU) void paged_attn_ke
         step *= kGroup;
       }
     }
-    __syncthreads();  // the area is free again
     g0 = ge;
+    if (kWhole || g0 >= g1) break;
+    __syncthreads();  // the area is free again
   }
 }
 
@@ -466,27 +538,17 @@ size_t paged_work_floats() { return static_cast<size_t>(2) * kMaxWg * slot_float
 size_t paged_cnt_words() { return static_cast<size_t>(6) * kMaxWg; }
 
 void launch_paged_attn(const PagedAttn &a, float *work, unsigned *cnt, hipStream_t s) {
-  Params p{a, work, cnt, a.hq / a.kv.hkv, 0, 0, 0, XE_PA_L};
+  Params p{a, work, cnt, a.hq / a.kv.hkv, 0, 0, 0};
   p.blocks = (p.group + kRows - 1) / kRows;
   p.rows = std::min(p.group, kRows);
   p.slot_floats = static_cast<unsigned>(slot_floats_of(a.kv.hd, p.rows));
   const int64_t cap = static_cast<int64_t>(a.kv.max_pages) << a.kv.page_shift;
   const int64_t units = static_cast<int64_t>(a.kv.batch) * a.kv.hkv * p.blocks;
   XE_REQUIRE(cap / kTile * units < (int64_t(1) << 31), "paged attention: more than 2^31 blocks of 16 keys in the table");
-#ifdef XE_PA_FEW
-  const bool wide = units < XE_PA_FEW;
-#else
-  const bool wide = units < 64;
-#endif
-#ifndef XE_PA_WG4
-#define XE_PA_WG4 512
-#endif
-#ifndef XE_PA_WG8
-#define XE_PA_WG8 256
-#endif
+  const bool wide = units < kManyUnits;
   const int kw = wide ? 8 : 4;
-  const int64_t wgs = std::max<int64_t>(1, std::min<int64_t>(wide ? XE_PA_WG8 : XE_PA_WG4, cap / kTile * units));
-  const size_t lds = area_bytes(a.kv.hd, p.rows, kw) + 4 * static_cast<size_t>(a.kv.batch);
+  const int64_t wgs = std::max<int64_t>(1, std::min<int64_t>(std::min(kMaxWg, (wide ? 1 : 2) * gdev::cu_count()), cap / kTile * units));
+  const size_t lds = area_bytes(a.kv.hd, p.rows, kw) + 8 * static_cast<size_t>(a.kv.batch);
   const PagedFn fn = wide ? pick<8>(a.kv.hd) : pick<4>(a.kv.hd);
   if (lds > 64 * 1024)
     XE_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));

@@ -43,20 +43,44 @@ XE_HD unsigned granules(int lo, int hi, int kg) {
 }
 
 // The granules of all units -- unit (stream, block of query heads), stream by
-// stream -- in a row, [0, total), are shared out in equal ranges: workgroup i
-// takes [i * per, (i + 1) * per).
-XE_HD unsigned share_of(unsigned total, unsigned workgroups, unsigned least) {
-  const unsigned per = (total + workgroups - 1) / workgroups;
-  return per < least ? least : per;
+// stream -- lie in a row, [0, total), and workgroup i takes [i * per, (i + 1) *
+// per): equal shares, from the middle of one unit to the middle of another.
+XE_HD unsigned share_of(unsigned total, unsigned workgroups) { return (total + workgroups - 1) / workgroups; }
+
+// Whole quotients by a divisor that is used often: m = floor((2^32 - 1) / d)
+// gives floor(n / d) or one less.
+struct Div {
+  unsigned d, m;
+};
+XE_HD Div div_by(unsigned d) { return Div{d, 0xffffffffu / d}; }
+XE_HD unsigned quot(unsigned n, const Div &v) {
+  const unsigned q = static_cast<unsigned>((static_cast<unsigned long long>(n) * v.m) >> 32);
+  return q + (n - q * v.d >= v.d ? 1u : 0u);
+}
+XE_HD unsigned quot_up(unsigned n, const Div &v) {
+  const unsigned q = quot(n, v);
+  return q + (q * v.d != n ? 1u : 0u);
 }
 
-// Workgroups that the unit of granules [u0, u1) is spread over: first_wg(u0)
-// and the ones behind it.
-XE_HD unsigned first_wg(unsigned u0, unsigned per) { return u0 / per; }
-XE_HD unsigned wg_count(unsigned u0, unsigned u1, unsigned per) { return (u1 - 1) / per - u0 / per + 1; }
+// Whole workgroups a unit: workgroup i of the `wgs` that share a unit of n
+// granules takes [t0, t1), as equal as can be.
+XE_HD void part_of(unsigned n, unsigned wgs, unsigned i, unsigned &t0, unsigned &t1) {
+  const unsigned q = n / wgs, r = n - q * wgs;
+  t0 = q * i + (i < r ? i : r);
+  t1 = t0 + q + (i < r ? 1u : 0u);
+}
+// Granules a workgroup takes at least, so that units of up to `alone` stay in
+// one and the longest needs no second level of groups of partials where `more`
+// a workgroup avoid it.
+XE_HD unsigned least_share(unsigned longest, unsigned group, unsigned alone, unsigned more) {
+  if (longest <= alone) return longest;
+  const unsigned q = (longest + group - 1) / group;
+  return q <= more ? (q < more / 3 ? more / 3 : q) : 1;
+}
 
-// Place of workgroup wg's partial of that unit: a workgroup has at most one
-// unit that began before it and one that it begins and does not end.
+// Place of workgroup wg's partial of the unit that begins at granule u0: a
+// workgroup has at most one unit that began before it and one that it begins
+// and does not end.
 XE_HD unsigned slot_of(unsigned u0, unsigned per, unsigned wg) { return 2 * wg + (u0 >= wg * per ? 1u : 0u); }
 
 }  // namespace paged
