@@ -98,18 +98,35 @@ int main() {
     const unsigned nwg = pick(2) ? 256 : 1 + pick(512), per = share_of(total, nwg);
     const Div by = div_by(per);
     assert(per >= 1 && (unsigned long long)per * nwg >= total);
+    const unsigned slack = pick(3) ? pick(20) : pick(200);
+    std::vector<unsigned> begin(nwg + 1, total);  // of each share
+    {
+      unsigned u0 = 0, i = 0;
+      for (int u = 0; u < units; u0 += n[u++])
+        for (; i <= nwg && i * per < u0 + n[u]; i++) begin[i] = snapped(i * per, u0, n[u], slack);
+      for (unsigned k = 0; k < nwg; k++) assert(begin[k] <= begin[k + 1]);
+      assert(begin[0] == 0 && begin[nwg] == total);
+    }
     std::set<unsigned> places;
     unsigned u0 = 0, covered = 0;
     for (int u = 0; u < units; u++) {
-      const unsigned u1 = u0 + n[u], w0 = quot(u0, by), cnt = quot(u1 - 1, by) - w0 + 1;
-      assert(cnt >= 1 && w0 + cnt <= nwg);
-      for (unsigned wg = w0; wg < w0 + cnt; wg++) {
-        const unsigned a = wg * per > u0 ? wg * per : u0, z = (wg + 1) * per < u1 ? (wg + 1) * per : u1;
-        assert(a < z);
+      const unsigned u1 = u0 + n[u];
+      unsigned w0 = ~0u, cnt = 0, has = 0, first = 0;
+      for (unsigned wg = 0; wg < nwg; wg++) {
+        const unsigned a = begin[wg] > u0 ? begin[wg] : u0, z = begin[wg + 1] < u1 ? begin[wg + 1] : u1;
+        if (a >= z) continue;
+        if (!has++) first = wg;
+        assert(wg == first + has - 1);
         covered += z - a;
-        const unsigned slot = slot_of(u0, per, wg);
-        assert(slot < 2 * nwg);
-        if (cnt > 1) assert(places.insert(slot).second);
+      }
+      spread(u0, n[u], by, slack, w0, cnt);
+      assert(cnt == has);
+      if (cnt > 1) {
+        assert(w0 == first && w0 + cnt <= nwg);
+        for (unsigned wg = w0; wg < w0 + cnt; wg++) {
+          const unsigned slot = slot_of(u0, per, wg);
+          assert(slot < 2 * nwg && places.insert(slot).second);
+        }
       }
       u0 = u1;
     }

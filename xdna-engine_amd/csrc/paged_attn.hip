@@ -6,21 +6,21 @@
 // Bound by the bytes of the keys and values: 4 hd a key and kv head against
 // 4 hd operations a query head.  What it takes to come near that:
 //
-// * Equal shares.  Streams differ in length, so the keys of all (stream,
-//   block of up to 16 query heads of a kv head) units are cut into granules of
-//   256 keys, and every workgroup takes the same number of granules in a row,
-//   from the middle of one unit to the middle of another (paged_index.h).  The
-//   lengths are on the device, so each workgroup sums them up itself.
-// * Everything in registers.  A wave takes 32 keys at a time.  Scores come out
-//   transposed, S^T = K Q^T (v_mfma_f32_16x16x32_bf16, 16 keys as A), so a lane
+// * Shares.  Streams differ in length, so the keys of all units -- (stream,
+//   block of up to 16 query heads of a kv head) -- are counted in tiles of 16
+//   and shared out equally: few units by whole workgroups, many in one row, from
+//   the middle of one unit to the middle of another (below, paged_index.h).  The
+//   lengths are on the device, so each workgroup counts them itself.
+// * Everything in registers.  A wave takes 16 keys at a time.  Scores come out
+//   transposed, S^T = K Q^T (v_mfma_f32_16x16x32_bf16, the keys as A), so a lane
 //   holds keys 4 g .. + 3 (g = lane / 16) of query row lane % 16: as they are,
-//   the B operand of O^T = V^T P^T with k slot 8 g + j read as key 4 g + j of
-//   the first 16 keys (j < 4) or of the second.  For its A operand a lane loads
-//   16 bytes -- 8 dimensions -- of each of its 8 keys, whole rows a load, and
-//   turns the 8 x 8 block with byte permutes: MFMA e takes dimension 8 n + e as
-//   row n.  No LDS and no barrier between a unit's first and last key; the next
-//   keys load while the values are multiplied, the next values during the next
-//   scores.
+//   the B operand of O^T = V^T P^T (v_mfma_f32_16x16x16_bf16).  For its A operand
+//   a lane loads 16 bytes -- 8 dimensions -- of each of these 4 keys, whole rows
+//   a load, and turns the block with byte permutes: MFMA e takes dimension 8 n +
+//   e as row n.  No LDS for keys and values and no barrier between a unit's
+//   first and last key; the next keys load while the values are multiplied, the
+//   next values during the next scores, and no load of either hangs on a branch
+//   (one that did made every wait one for both: 118 us for 113).
 // * fp32 results.  Queries and probabilities are three bf16 parts each, exact
 //   (8 bits a part); keys and values are bf16 as stored; scores, softmax
 //   statistics and sums are fp32, the softmax with a running maximum, base 2.
@@ -47,16 +47,26 @@ constexpr int kRows = 16;    // query heads a unit at most
 constexpr int kMaxWg = 512;
 constexpr int kGroup = 16;   // partials merged at once
 constexpr int kMaxHd = 256;
-// Fewer units than this: workgroups of eight waves, one a CU, whole ones a
-// unit, so that a workgroup has one unit's chain of loads before it; else of
-// four, two a CU, in equal shares.  us with eight / four waves: 32768 keys of
-// one stream (4 x 256) 19.7 / 23.6, 60000 keys (7 x 128) 16.7 / 21.1, 8 mixed
-// streams to 3000 keys (8 / 2 x 128, 16 units) 10.9 / 10.8, 64 streams to 4096
-// (4 x 256, 64 units) 50.3 / 46.9, 192 mixed to 5000 (6 / 2 x 64) 59.6 / 54.3.
-// Nontemporal loads where the keys are many, us plain / nontemporal: 150 mixed
-// streams to 8192 keys (16 / 2 x 128) 113 / 103, 48 to 8192 (12 x 64) 159 / 145;
-// 32768 keys of one stream 19.7 / 20.3.
+// Two forms.  Workgroups of eight waves, one a CU, whole ones a unit, so that a
+// workgroup has one unit's chain of loads before it: up to 64 streams of up to
+// a unit a CU, of fewer than kManyUnits units or of keys (those the table or
+// the window allows) up to kFewBytes.  Else of four waves, two a CU, in equal
+// shares of all keys, with nontemporal loads.  us with the first / the second:
+// 32768 keys of one stream (4 x 256) 18.2 / 23.6, 8 mixed streams to 3000 keys
+// (8 / 2 x 128) 9.7 / 10.8, 32 of window 1024 12.5 / 16.5, 60 to 300 keys (16 /
+// 4 x 128) 9.4 / 13.6, 64 to 1500 (4 x 256) 20.9 / 26.5, 64 to 4096 50.3 / 46.1.
+// Nontemporal loads, us plain / nontemporal: 150 mixed streams to 8192 keys
+// (16 / 2 x 128) 113 / 103, 48 to 8192 (12 x 64) 159 / 145; 32768 keys of one
+// stream 19.7 / 20.3.
 constexpr int kManyUnits = 64;
+constexpr int64_t kFewBytes = int64_t(128) << 20;
+// Equal shares: a unit counts kStart4 tiles on top of its own, about what its
+// chain of loads before the first tile and the meeting after the last cost, and
+// none is cut within kSlack of its ends.  us without / with: 128 mixed streams
+// to 300 keys (12 x 64) 65 / 24, 192 to 5000 (6 / 2 x 64) 51.4 / 46.0; 16 and 16
+// take 64 streams to 4096 (4 x 256) from 45.9 to 52.7.
+constexpr unsigned kStart4 = 8, kSlack = 8;
+static_assert(kSlack >= kStart4, "no share begins among what a unit counts on top");
 // Whole workgroups a unit: units of up to kAlone tiles in one workgroup (28
 // tiles, 12 units of hd 64: 7.7 us, in two workgroups each 8.9), up to kMore
 // tiles a workgroup where a second level of merges is avoided with them (188
@@ -154,6 +164,7 @@ template <int HD, int KW>
 __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(Params p) {
   constexpr int T = 64 * KW;
   constexpr bool kWhole = KW == 8;          // whole workgroups a unit; else equal shares of all keys
+  constexpr unsigned kStart = kWhole ? 0 : kStart4;  // granules that a unit counts on top of its own
   constexpr bool kStream = KW == 4;         // keys and values by nontemporal loads
   constexpr int S = HD / 32;                // 32-dimension steps of a score
   constexpr int VB = HD >= 128 ? 8 : 4;     // dimensions of a value a lane loads at once
@@ -162,7 +173,7 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(Params p) {
   typedef unsigned VReg __attribute__((ext_vector_type(VB / 2)));
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   __shared__ unsigned scan[KW + 1];
-  __shared__ unsigned found[4];
+  __shared__ unsigned found[5];
   unsigned char *const qs = lds;                                              // [3][S][64] x 16 bytes
   float *const meet = reinterpret_cast<float *>(lds);                         // [KW][rows][HD], m and l [KW][kRows]
   int32_t *const lens = reinterpret_cast<int32_t *>(lds + area_bytes(HD, p.rows, KW));  // [batch]
@@ -186,7 +197,7 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(Params p) {
     const unsigned n = paged::granules(lo, hi, kTile);
     lens[b] = len;
     count[b] = n;
-    mine += n;
+    mine += n ? n + kStart : 0;
   }
   const unsigned incl = wave_scan(mine * H);
   unsigned before = incl - mine * H, total = __builtin_amdgcn_readlane(incl, 63);
@@ -210,7 +221,7 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(Params p) {
 
   paged::Div per = paged::div_by(paged::share_of(total, nwg));
   unsigned g0 = wg * per.d;
-  const unsigned g1 = min(g0 + per.d, total);
+  unsigned g1 = 0;
   int b = 0;                                   // stream
   unsigned base = 0;                           // its first granule
   unsigned wgs = 0, part = 0, part_unit = 0;   // kWhole: the unit's workgroups, this one among them, the unit
@@ -235,16 +246,32 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(Params p) {
     part = at - part_unit * wgs;
   } else {
     if (g0 >= total) return;
-    if (g0 >= before && g0 < before + mine * H) {
+    // where the shares of this workgroup and of the next begin
+    if (tid == 0) found[3] = total;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const unsigned g = (wg + i) * per.d;
+      if (g < before || g >= before + mine * H) continue;
       unsigned sum = before;
       int s = s0;
-      for (; g0 >= sum + count[s] * H; s++) sum += count[s] * H;
-      found[0] = s;
-      found[1] = sum;
+      for (;; s++) {
+        const unsigned n = count[s] ? (count[s] + kStart) * H : 0;
+        if (g < sum + n) break;
+        sum += n;
+      }
+      found[2 + i] = paged::snapped(g, sum, count[s] + kStart, kSlack);
+      if (i == 0) {
+        found[0] = s;
+        found[1] = sum;
+      }
     }
     __syncthreads();
     b = __builtin_amdgcn_readfirstlane(found[0]);
     base = __builtin_amdgcn_readfirstlane(found[1]);
+    g0 = __builtin_amdgcn_readfirstlane(found[2]);
+    g1 = __builtin_amdgcn_readfirstlane(found[3]);
+    if (g0 >= g1) return;
   }
   const float sc2 = p.a.scale * adev::kLog2e;
   const size_t head_rows = static_cast<size_t>(1) << kv.page_shift;
@@ -256,7 +283,7 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(Params p) {
     const int ln = own & 15, lg = (own >> 4) & 3;
     int lo, hi;
     paged::key_range(__builtin_amdgcn_readfirstlane(lens[b]), p.a.window, cap, lo, hi);
-    const unsigned n = __builtin_amdgcn_readfirstlane(count[b]);
+    const unsigned real = __builtin_amdgcn_readfirstlane(count[b]), n = real ? real + kStart : 0;
     unsigned unit = part_unit, u0 = ~0u, ge = g1;  // partials in slots 2 i + 1
     unsigned w0 = wg - part, nseg = wgs, t0, t1;   // the unit's workgroups, this one's granules of it
     if constexpr (kWhole) {
@@ -270,10 +297,9 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(Params p) {
       unit = (g0 - base) / n;
       u0 = base + unit * n;
       ge = min(g1, u0 + n);
-      w0 = paged::quot(u0, per);
-      nseg = paged::quot(u0 + n - 1, per) - w0 + 1;
-      t0 = g0 - u0;
-      t1 = ge - u0;
+      paged::spread(u0, n, per, kSlack, w0, nseg);
+      t0 = g0 == u0 ? 0 : g0 - u0 - kStart;
+      t1 = ge - u0 - kStart;
     }
     const int kvh = unit / p.blocks, r0 = (unit - kvh * p.blocks) * kRows;
     const int rows = min(p.group - r0, kRows), h0 = kvh * p.group + r0;
@@ -476,7 +502,7 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(Params p) {
         const bool final = left <= kGroup;
         unsigned *const counter = p.cnt + (step == 1 ? 0 : step == kGroup ? 2 * kMaxWg : 4 * kMaxWg) +
                                   paged::slot_of(u0, per.d, w0 + seg0 * step);
-        const bool last = adev::last_to_arrive(counter, static_cast<int>(cnt), reinterpret_cast<int *>(found + 2));
+        const bool last = adev::last_to_arrive(counter, static_cast<int>(cnt), reinterpret_cast<int *>(found + 4));
         if (!last) break;
         if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         const unsigned dst = paged::slot_of(u0, per.d, w0 + seg0 * step) * p.slot_floats;
@@ -545,7 +571,8 @@ void launch_paged_attn(const PagedAttn &a, float *work, unsigned *cnt, hipStream
   const int64_t cap = static_cast<int64_t>(a.kv.max_pages) << a.kv.page_shift;
   const int64_t units = static_cast<int64_t>(a.kv.batch) * a.kv.hkv * p.blocks;
   XE_REQUIRE(cap / kTile * units < (int64_t(1) << 31), "paged attention: more than 2^31 blocks of 16 keys in the table");
-  const bool wide = units < kManyUnits;
+  const int64_t span = a.window ? std::min<int64_t>(cap, static_cast<int64_t>(a.window) + kTile) : cap;
+  const bool wide = a.kv.batch <= 64 && units <= gdev::cu_count() && (units < kManyUnits || units * span * a.kv.hd * 4 <= kFewBytes);
   const int kw = wide ? 8 : 4;
   const int64_t wgs = std::max<int64_t>(1, std::min<int64_t>(std::min(kMaxWg, (wide ? 1 : 2) * gdev::cu_count()), cap / kTile * units));
   const size_t lds = area_bytes(a.kv.hd, p.rows, kw) + 8 * static_cast<size_t>(a.kv.batch);

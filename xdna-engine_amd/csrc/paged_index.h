@@ -78,6 +78,26 @@ XE_HD unsigned least_share(unsigned longest, unsigned group, unsigned alone, uns
   return q <= more ? (q < more / 3 ? more / 3 : q) : 1;
 }
 
+// Shares begin at i * per, or at the end of a unit that lies at most `slack`
+// granules from there: neither a unit of few granules nor an end of one is
+// split off for its sake.  g lies in a unit of n granules of the stream that
+// begins at granule base.
+XE_HD unsigned snapped(unsigned g, unsigned base, unsigned n, unsigned slack) {
+  const unsigned off = (g - base) % n;
+  return off <= slack && off <= n - off ? g - off : n - off <= slack ? g - off + n : g;
+}
+// Workgroups that the unit of granules [u0, u0 + n) is spread over: wgs of
+// them, from w0 on (wgs = 1: the one whose share it lies in, w0 is not set).
+XE_HD void spread(unsigned u0, unsigned n, const Div &per, unsigned slack, unsigned &w0, unsigned &wgs) {
+  wgs = 1;
+  if (n <= 2 * slack) return;
+  // shares that begin within it, further than slack from its ends
+  const unsigned a = quot(u0 + slack, per) + 1, z = quot(u0 + n - slack - 1, per);
+  if (z < a) return;
+  w0 = a - 1;
+  wgs = z - a + 2;
+}
+
 // Place of workgroup wg's partial of the unit that begins at granule u0: a
 // workgroup has at most one unit that began before it and one that it begins
 // and does not end.
