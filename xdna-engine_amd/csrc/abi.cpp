@@ -114,15 +114,24 @@ char *xe_ctx::ensure_w8a8(size_t aq_bytes) {
   return w8a8_ws;
 }
 
-char *xe_ctx::ensure_rows(size_t n) {
-  if (n > rows_ws_size) {
-    if (rows_ws) XE_HIP(hipFree(rows_ws));
-    rows_ws = nullptr;
-    rows_ws_size = 0;
-    XE_HIP(hipMalloc(&rows_ws, n));
-    rows_ws_size = n;
+static constexpr size_t kRowsPart = 2048 + 4096;  // where rows_ws holds partial tiles
+
+void xe_ctx::ensure_rows(size_t codes_bytes) {
+  if (!rows_ws) {
+    char *ws = nullptr;
+    XE_HIP(hipMalloc(&ws, rows_q8_ws_bytes()));
+    const hipError_t e = hipMemsetAsync(ws, 0, kRowsPart, dev->stream);
+    if (e != hipSuccess) (void)hipFree(ws);
+    XE_HIP(e);
+    rows_ws = ws;
   }
-  return rows_ws;
+  if (codes_bytes > rows_codes_size) {
+    if (rows_codes) XE_HIP(hipFree(rows_codes));
+    rows_codes = nullptr;
+    rows_codes_size = 0;
+    XE_HIP(hipMalloc(&rows_codes, codes_bytes));
+    rows_codes_size = codes_bytes;
+  }
 }
 
 void xe_ctx::ensure_paged() {
@@ -532,6 +541,7 @@ void xe_ctx_destroy(xe_ctx *ctx) {
     if (ctx->gemm_xn) (void)hipFree(ctx->gemm_xn);
     if (ctx->w8a8_ws) (void)hipFree(ctx->w8a8_ws);
     if (ctx->rows_ws) (void)hipFree(ctx->rows_ws);
+    if (ctx->rows_codes) (void)hipFree(ctx->rows_codes);
     if (ctx->paged_work) (void)hipFree(ctx->paged_work);
     if (ctx->paged_cnt) (void)hipFree(ctx->paged_cnt);
     delete ctx;
@@ -1148,9 +1158,11 @@ int xe_w8a8_rows_dev(xe_ctx *ctx, const xe_weight *w, const xe_w8a8_rows *rows) 
     r.beta = w->beta;
     r.eps = w->eps;
     r.a = *rows;
-    char *ws = ctx->ensure_rows(2048 + static_cast<size_t>(rows->batch) * w->k);
-    r.scales = reinterpret_cast<float *>(ws);
-    r.codes = reinterpret_cast<int8_t *>(ws + 2048);
+    ctx->ensure_rows(rows_q8_codes_bytes(rows->batch, w->k));
+    r.scales = reinterpret_cast<float *>(ctx->rows_ws);
+    r.cnt = reinterpret_cast<unsigned *>(ctx->rows_ws + 2048);
+    r.part = reinterpret_cast<int *>(ctx->rows_ws + kRowsPart);
+    r.codes = reinterpret_cast<int8_t *>(ctx->rows_codes);
     launch_rows_q8(r, ctx->dev->stream);
     ctx->dispatches += 2;
     return 0;

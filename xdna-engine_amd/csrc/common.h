@@ -101,10 +101,12 @@ struct xe_ctx {
   char *w8a8_ws = nullptr;
   size_t w8a8_ws_size = 0;
   char *ensure_w8a8(size_t aq_bytes);
-  // int8 linears with a scale a row: the scales and the codes
+  // int8 linears with a scale a row: scales, arrival counters (zeroed once,
+  // self-resetting) and partial tiles, allocated by the first call; the codes
   char *rows_ws = nullptr;
-  size_t rows_ws_size = 0;
-  char *ensure_rows(size_t n);
+  char *rows_codes = nullptr;
+  size_t rows_codes_size = 0;
+  void ensure_rows(size_t codes_bytes);
   // attention over pages: partials and arrival counters (zeroed once,
   // self-resetting), allocated by the first call
   float *paged_work = nullptr;

@@ -37,8 +37,9 @@ size_t paged_work_floats();
 size_t paged_cnt_words();
 
 // y = act((q . w) s ws + bias) + res over the int8 codes q of norm(x + add)
-// and their row scales s; codes / scales: workspace, batch * k bytes and batch
-// floats.
+// and their row scales s; codes / scales: workspace, rows_q8_codes_bytes() and
+// batch floats.  kp, vec: set by the launch (a row of codes with its padding,
+// whether results go out 16 bytes at a time).
 struct RowsQ8 {
   const int8_t *w = nullptr;
   const float *ws = nullptr, *bias = nullptr;
@@ -48,7 +49,14 @@ struct RowsQ8 {
   xe_w8a8_rows a{};
   int8_t *codes = nullptr;
   float *scales = nullptr;
+  int *part = nullptr;
+  unsigned *cnt = nullptr;
+  int kp = 0, vec = 0;
 };
+size_t rows_q8_codes_bytes(int batch, int k);
+// Scales (2 KB), then arrival counters (4 KB, zeroed once; they re-arm), then
+// partial tiles of K splits.
+size_t rows_q8_ws_bytes();
 void launch_rows_q8(const RowsQ8 &r, hipStream_t s);
 
 }  // namespace xe

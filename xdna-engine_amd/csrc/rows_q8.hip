@@ -6,117 +6,203 @@
 // on the streams beside it (xe_w8a8_linear has one scale for all rows).
 // Statistics and rounding are in fp64, so that a code between two values does
 // not depend on the order of a sum: q and s are those of h itself.
-#include "gemv_dev.h"
+#include "attn_dev.h"
 #include "paged.h"
 
 namespace xe {
 namespace {
 
 constexpr int kT = 256;
-constexpr int kNoRec = 0x7ffffff0;  // past every buffer: loads return zeros
+constexpr unsigned kNoRec = 0x7ffffff0u;  // past every buffer: loads return zeros
+
+constexpr int kXcds = 8;
+constexpr size_t kPartBytes = size_t(32) << 20;  // partial tiles of K splits
+constexpr size_t kCntWords = 1024;               // and their arrival counters
+constexpr int kStep = 128;          // bytes of K a step
+constexpr int kFusedBytes = 8192;   // codes that a workgroup makes itself
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
-  return v;
-}
-__device__ __forceinline__ double wave_max64(double v) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v = fmax(v, __shfl_xor(v, off, 64));
-  return v;
+// Raw buffer over `bytes` bytes: loads past its end give zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t bounded_rsrc(const void *base, unsigned bytes) {
+  const uint64_t a = reinterpret_cast<uint64_t>(base);
+  const uint64_t lo = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a)));
+  const uint64_t hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a >> 32)));
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>(hi << 32 | lo), static_cast<short>(0),
+                                           static_cast<int>(__builtin_amdgcn_readfirstlane(bytes)), 0x00020000);
 }
 
+// A double moved by a 32-bit lane move of its halves.
 template <typename F>
-__device__ __forceinline__ double block_reduce(double v, double *red, F op) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  __syncthreads();
-  if (lane == 0) red[wave] = v;
+__device__ __forceinline__ double moved(double v, F &&move) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = move(static_cast<uint32_t>(u)), hi = move(static_cast<uint32_t>(u >> 32));
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double v) {
+  return moved(v, [](uint32_t x) { return static_cast<uint32_t>(gdev::dpp_get_i<CTRL>(static_cast<int>(x))); });
+}
+template <bool HALF>  // the value of the other 32 lanes (HALF) or of the neighbouring 16
+__device__ __forceinline__ double other64(double v) {
+  return moved(v, [](uint32_t x) {
+    const auto r = HALF ? __builtin_amdgcn_permlane32_swap(x, x, false, false) : __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return (threadIdx.x & (HALF ? 32 : 16)) ? r[0] : r[1];
+  });
+}
+// op over all threads of the workgroup, the same in each; red: T / 64 doubles
+// of a slot that no wave still reads.
+template <int T, typename Op>
+__device__ __forceinline__ double block_all(double v, double *red, Op op) {
+  v = op(v, dpp64<gdev::kDppXor1>(v));
+  v = op(v, dpp64<gdev::kDppXor2>(v));
+  v = op(v, dpp64<gdev::kDppHalfMirror>(v));
+  v = op(v, dpp64<gdev::kDppMirror>(v));
+  v = op(v, other64<false>(v));
+  v = op(v, other64<true>(v));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
   v = red[0];
-  for (int w = 1; w < static_cast<int>(blockDim.x >> 6); w++) v = op(v, red[w]);
+#pragma unroll
+  for (int w = 1; w < T / 64; w++) v = op(v, red[w]);
   return v;
 }
+struct Sum64 {
+  __device__ double operator()(double a, double b) const { return a + b; }
+};
+struct Max64 {
+  __device__ double operator()(double a, double b) const { return fmax(a, b); }
+};
 
-// One workgroup a row; a thread holds elements threadIdx.x + T j.
-template <int NE, int T>
-__global__ __launch_bounds__(T) void rows_quant_kernel(RowsQ8 p) {
-  __shared__ double red[T / 64];
-  const int b = blockIdx.x, K = p.k;
-  const float *x = p.a.x + static_cast<size_t>(b) * K;
-  const float *add = p.a.add ? p.a.add + static_cast<size_t>(b) * K : nullptr;
-  auto sum = [](double u, double v) { return u + v; };
-  float t[NE], su[NE];
+template <bool VEC>
+__device__ __forceinline__ f32x4 load4(const float *p) {
+  if constexpr (VEC) return *reinterpret_cast<const f32x4 *>(p);
+  else return f32x4{p[0], p[1], p[2], p[3]};
+}
+
+// Codes lie as the matrix instruction takes them: a block of 1 KB for 64 k of 16
+// rows, [kp / 64][groups of 16 rows][4 x 16 k][16 rows][16 k], zeros behind K.  A
+// wave loads such an operand as one run of memory (112 B/ns a CU out of L2, 37
+// where 16 rows of 64 bytes lie apart); rows behind the last one are whatever is
+// there, and so are the results that nobody takes.
+__host__ __device__ __forceinline__ int row_groups(int batch) { return (batch + 15) / 16; }
+__device__ __forceinline__ size_t code_at(const RowsQ8 &p, int b, int i) {
+  return ((static_cast<size_t>(i / 64) * row_groups(p.a.batch) + b / 16) * 64 + i % 64 / 16 * 16 + b % 16) * 16 + i % 16;
+}
+
+// Row b to codes by T threads, a thread holding elements 4 (tid + T j) .. + 3:
+// put(i, four codes) for each four below kp, the scale returned.  `sum` is
+// written where `writes`.  red: four slots, not those of the row before.
+template <int NV, int T, bool VEC, typename Put>
+__device__ __forceinline__ float quant_row(const RowsQ8 &p, int b, bool writes, double (*red)[T / 64], Put &&put) {
+  const int K = p.k, tid = threadIdx.x;
+  const size_t at = static_cast<size_t>(b) * K;
+  f32x4 t[NV], su[NV], g[NV], be[NV];
 #pragma unroll
-  for (int j = 0; j < NE; j++) {
-    const int i = threadIdx.x + j * T;
-    t[j] = i < K ? x[i] : 0.f;
-    su[j] = add && i < K ? add[i] : 0.f;
+  for (int j = 0; j < NV; j++) {
+    const int i = 4 * (tid + T * j);
+    t[j] = su[j] = g[j] = be[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (i >= K) continue;
+    t[j] = load4<VEC>(p.a.x + at + i);
+    if (p.a.add) su[j] = load4<VEC>(p.a.add + at + i);
+    if (p.a.post_w) be[j] = load4<VEC>(p.a.post_w + i);
   }
   if (p.a.post_w) {
-    double s = 0.0;
+    double v = 0.0;
 #pragma unroll
-    for (int j = 0; j < NE; j++) s += static_cast<double>(su[j]) * su[j];
-    const double inv = 1.0 / sqrt(block_reduce(wave_sum64(s), red, sum) / K + static_cast<double>(p.a.post_eps));
+    for (int j = 0; j < NV; j++)
 #pragma unroll
-    for (int j = 0; j < NE; j++) {
-      const int i = threadIdx.x + j * T;
-      if (i < K) su[j] = static_cast<float>(su[j] * inv * (1.0 + p.a.post_w[i]));
+      for (int c = 0; c < 4; c++) v += static_cast<double>(su[j][c]) * su[j][c];
+    const double inv = 1.0 / sqrt(block_all<T>(v, red[0], Sum64{}) / K + static_cast<double>(p.a.post_eps));
+#pragma unroll
+    for (int j = 0; j < NV; j++)
+#pragma unroll
+      for (int c = 0; c < 4; c++) su[j][c] = static_cast<float>(su[j][c] * inv * (1.0 + be[j][c]));
+  }
+#pragma unroll
+  for (int j = 0; j < NV; j++) {
+    const int i = 4 * (tid + T * j);
+    if (i >= K) continue;
+    if (p.a.add)
+#pragma unroll
+      for (int c = 0; c < 4; c++) t[j][c] += su[j][c];
+    if (p.a.sum && writes) {
+      if constexpr (VEC) *reinterpret_cast<f32x4 *>(p.a.sum + at + i) = t[j];
+      else
+#pragma unroll
+        for (int c = 0; c < 4; c++) p.a.sum[at + i + c] = t[j][c];
     }
+    if (p.norm != XE_NORM_NONE) g[j] = *reinterpret_cast<const f32x4 *>(p.gamma + i);
+    if (p.norm == XE_NORM_LN) be[j] = *reinterpret_cast<const f32x4 *>(p.beta + i);
   }
-  double h[NE];
-#pragma unroll
-  for (int j = 0; j < NE; j++) {
-    const int i = threadIdx.x + j * T;
-    if (add) t[j] += su[j];
-    if (p.a.sum && i < K) p.a.sum[static_cast<size_t>(b) * K + i] = t[j];
-    h[j] = t[j];
-  }
+  double mean = 0.0, inv = 1.0;
+  const double one = p.norm == XE_NORM_RMS1P ? 1.0 : 0.0;
   if (p.norm != XE_NORM_NONE) {
-    double mean = 0.0;
+    double v = 0.0;
     if (p.norm == XE_NORM_LN) {
-      double s = 0.0;
 #pragma unroll
-      for (int j = 0; j < NE; j++) s += h[j];
-      mean = block_reduce(wave_sum64(s), red, sum) / K;
-    }
-    double s = 0.0;
+      for (int j = 0; j < NV; j++)
 #pragma unroll
-    for (int j = 0; j < NE; j++) {
-      const int i = threadIdx.x + j * T;
-      h[j] = i < K ? h[j] - mean : 0.0;
-      s += h[j] * h[j];
+        for (int c = 0; c < 4; c++) v += t[j][c];
+      mean = block_all<T>(v, red[1], Sum64{}) / K;
+      v = 0.0;
     }
-    const double inv = 1.0 / sqrt(block_reduce(wave_sum64(s), red, sum) / K + static_cast<double>(p.eps));
 #pragma unroll
-    for (int j = 0; j < NE; j++) {
-      const int i = threadIdx.x + j * T;
-      if (i >= K) continue;
-      h[j] = h[j] * inv * ((p.norm == XE_NORM_RMS1P ? 1.0 : 0.0) + p.gamma[i]);
-      if (p.norm == XE_NORM_LN) h[j] += p.beta[i];
-    }
+    for (int j = 0; j < NV; j++)
+#pragma unroll
+      for (int c = 0; c < 4; c++)
+        if (4 * (tid + T * j) < K) v += (t[j][c] - mean) * (t[j][c] - mean);
+    inv = 1.0 / sqrt(block_all<T>(v, red[2], Sum64{}) / K + static_cast<double>(p.eps));
   }
-  // NaN and infinity: the row's scale becomes NaN, and with it its outputs
+  auto h = [&](int j, int c) {
+    if (p.norm == XE_NORM_NONE) return static_cast<double>(t[j][c]);
+    const double v = (t[j][c] - mean) * inv * (one + g[j][c]);
+    return p.norm == XE_NORM_LN ? v + be[j][c] : v;
+  };
   double a = 0.0;
   bool bad = false;
 #pragma unroll
-  for (int j = 0; j < NE; j++) {
-    a = fmax(a, fabs(h[j]));
-    bad |= !(fabs(h[j]) <= 1.7976931348623157e308);
-  }
-  a = bad ? INFINITY : a;
-  const double amax = block_reduce(wave_max64(a), red, [](double u, double v) { return fmax(u, v); });
-  const float scale = amax > 0.0 ? static_cast<float>(amax / 127.0) : 1.0f;
-  if (threadIdx.x == 0) p.scales[b] = scale < INFINITY ? scale : NAN;
-  const double r = 1.0 / static_cast<double>(scale);
+  for (int j = 0; j < NV; j++)
 #pragma unroll
-  for (int j = 0; j < NE; j++) {
-    const int i = threadIdx.x + j * T;
-    if (i >= K) continue;
-    const double v = fmin(fmax(round(h[j] * r), -127.0), 127.0);
-    p.codes[static_cast<size_t>(b) * K + i] = scale < INFINITY ? static_cast<int8_t>(static_cast<int>(v)) : static_cast<int8_t>(0);
+    for (int c = 0; c < 4; c++) {
+      if (4 * (tid + T * j) >= K) continue;
+      const double v = fabs(h(j, c));
+      bad |= !(v <= 1.7976931348623157e308);
+      a = fmax(a, v);
+    }
+  const double amax = block_all<T>(bad ? INFINITY : a, red[3], Max64{});
+  float s = static_cast<float>(amax / 127.0);
+  if (!(s > 0.f)) s = 1.f;
+  const bool number = s < INFINITY;  // else NaN or infinity in the row: its scale, and its outputs, become NaN
+  const double r = 1.0 / static_cast<double>(s);
+#pragma unroll
+  for (int j = 0; j < NV; j++) {
+    const int i = 4 * (tid + T * j);
+    if (i >= p.kp) continue;
+    uint32_t q = 0;
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      const int code = static_cast<int>(fmin(fmax(round(h(j, c) * r), -127.0), 127.0));
+      q |= (static_cast<uint32_t>(code) & 0xffu) << (8 * c);
+    }
+    put(i, number && i < K ? q : 0u);
   }
+  return number ? s : NAN;
+}
+
+// One workgroup a row.  Bound by the rows' bytes where they are many, by the
+// chain of a load and two or three block reductions where they are few.
+template <int NV, int T, bool VEC>
+__global__ __launch_bounds__(T) void rows_quant_kernel(RowsQ8 p) {
+  __shared__ double red[4][T / 64];
+  const int b = blockIdx.x;
+  const float s = quant_row<NV, T, VEC>(p, b, true, red, [&](int i, uint32_t q) {
+    *reinterpret_cast<uint32_t *>(p.codes + code_at(p, b, i)) = q;
+  });
+  if (threadIdx.x == 0) p.scales[b] = s;
 }
 
 __device__ __forceinline__ float gelu_tanh_f(float x) {
@@ -130,53 +216,502 @@ __device__ __forceinline__ float activate(int act, float z) {
   return z;
 }
 
-// Four waves of 16 weight rows, 16 activation rows a workgroup.
-__global__ __launch_bounds__(kT) void rows_gemm_kernel(RowsQ8 p) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int r0 = blockIdx.x * 64 + wave * 16, b0 = blockIdx.y * 16;
-  const __amdgpu_buffer_rsrc_t rw = gdev::coherent_rsrc(p.w);
-  const __amdgpu_buffer_rsrc_t ra = gdev::coherent_rsrc(p.codes);
-  const int row = r0 + (lane & 15), b = b0 + (lane & 15), kl = 16 * (lane >> 4);
-  i32x4 acc = {0, 0, 0, 0};
-  for (int k0 = 0; k0 < p.k; k0 += 64) {
-    const bool ok = k0 + kl < p.k;
-    const i32x4 wa = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rw, row < p.m && ok ? row * p.k + k0 + kl : kNoRec, 0, 0));
-    const i32x4 xa = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(ra, b < p.a.batch && ok ? b * p.k + k0 + kl : kNoRec, 0, 0));
-    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(wa, xa, acc, 0, 0, 0);
-  }
-  if (b >= p.a.batch) return;
-  const float s = p.scales[b];
-  float z[4];
+// Outputs r .. r + 3 of activation row b from their sums: what they take is
+// loaded early (rows and weight rows past the last one: the last one's).
+struct Epi4 {
+  float s, ws[4], bi[4], e[4];
+  __device__ __forceinline__ void load(const RowsQ8 &p, int b, int r, bool scale) {
+    b = min(b, p.a.batch - 1);
+    const bool pairs = p.a.act == XE_ACT_GEGLU;
+    const int mo = pairs ? p.m / 2 : p.m;
+    if (scale) s = p.scales[b];
+    if (p.vec) {
+      r = min(r, p.m - 4);
+      const f32x4 w4 = *reinterpret_cast<const f32x4 *>(p.ws + r);
+      f32x4 b4 = {0.f, 0.f, 0.f, 0.f}, e4 = b4;
+      if (p.bias) b4 = *reinterpret_cast<const f32x4 *>(p.bias + r);
+      if (p.a.res && pairs) {
+        const f32x2 e2 = *reinterpret_cast<const f32x2 *>(p.a.res + static_cast<size_t>(b) * mo + r / 2);
+        e4[0] = e2[0];
+        e4[2] = e2[1];
+      } else if (p.a.res) {
+        e4 = *reinterpret_cast<const f32x4 *>(p.a.res + static_cast<size_t>(b) * mo + r);
+      }
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const int r = min(r0 + 4 * (lane >> 4) + i, p.m - 1);
-    z[i] = static_cast<float>(acc[i]) * s * p.ws[r];
-    if (p.bias) z[i] += p.bias[r];
-  }
-  const bool pairs = p.a.act == XE_ACT_GEGLU;
-  const int mo = pairs ? p.m / 2 : p.m;
+      for (int i = 0; i < 4; i++) {
+        ws[i] = w4[i];
+        bi[i] = b4[i];
+        e[i] = e4[i];
+      }
+      return;
+    }
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    if (pairs && (i & 1)) continue;
-    const int r = r0 + 4 * (lane >> 4) + i;
-    if (r >= p.m) continue;
-    float y = pairs ? gelu_tanh_f(z[i]) * z[i + 1 < 4 ? i + 1 : 3] : activate(p.a.act, z[i]);
-    const size_t o = static_cast<size_t>(b) * mo + (pairs ? r / 2 : r);
-    if (p.a.res) y += p.a.res[o];
-    p.a.y[o] = y;
+    for (int i = 0; i < 4; i++) {
+      const int ri = min(r + i, p.m - 1);
+      ws[i] = p.ws[ri];
+      bi[i] = p.bias ? p.bias[ri] : 0.f;
+      e[i] = p.a.res ? p.a.res[static_cast<size_t>(b) * mo + (pairs ? ri / 2 : ri)] : 0.f;
+    }
   }
+  __device__ __forceinline__ void finish(const RowsQ8 &p, int b, int r, const i32x4 &sum) const {
+    const bool pairs = p.a.act == XE_ACT_GEGLU;
+    const int mo = pairs ? p.m / 2 : p.m;
+    float y[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      y[i] = static_cast<float>(sum[i]) * s * ws[i];
+      if (p.bias) y[i] += bi[i];
+    }
+    if (pairs) {
+      y[0] = gelu_tanh_f(y[0]) * y[1];
+      y[2] = gelu_tanh_f(y[2]) * y[3];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++) y[i] = activate(p.a.act, y[i]);
+    }
+    if (p.a.res)
+#pragma unroll
+      for (int i = 0; i < 4; i++) y[i] += e[i];
+    float *d = p.a.y + static_cast<size_t>(b) * mo + (pairs ? r / 2 : r);
+    if (p.vec && pairs) {
+      *reinterpret_cast<f32x2 *>(d) = f32x2{y[0], y[2]};
+    } else if (p.vec) {
+      *reinterpret_cast<f32x4 *>(d) = f32x4{y[0], y[1], y[2], y[3]};
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (r + i < p.m && !(pairs && (i & 1))) d[pairs ? i / 2 : i] = y[i];
+    }
+  }
+};
+
+// Tiles of WR x 16 weight rows and NJ x 16 activation rows a workgroup, its KS
+// waves each over their own part of K (v_mfma_i32_16x16x64_i8: a lane holds 16
+// consecutive k of weight row lane % 16 and of activation row lane % 16), U
+// steps of 64 in flight.  NV > 0: the workgroup makes the codes itself (K <= 1024
+// NV), into LDS, while its first weights load.
+template <int WR, int NJ, int KS, int U, int NV>
+__global__ __launch_bounds__(64 * KS) void rows_gemm_kernel(RowsQ8 p, int ntile_m, int ntile_b) {
+  constexpr int NB = WR * NJ;                     // 16 x 16 blocks
+  constexpr bool kFused = NV > 0;
+  static_assert(!kFused || (KS == 4 && NJ == 1), "rows made here: 256 threads, 16 rows at most");
+  __shared__ __attribute__((aligned(16))) int part[KS][NB][256];
+  __shared__ __attribute__((aligned(16))) int8_t codes[kFused ? kFusedBytes : 16];
+  __shared__ double red[kFused ? 8 : 1][4];
+  __shared__ float made[16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ln = lane & 15, lg = lane >> 4;
+  // The tiles of an XCD lie in a row, those of the same weight rows next to
+  // each other: its L2 reads the weights once.
+  const int all = ntile_m * ntile_b, each = (all + kXcds - 1) / kXcds;
+  const int tile = static_cast<int>(blockIdx.x % kXcds) * each + static_cast<int>(blockIdx.x / kXcds);
+  if (static_cast<int>(blockIdx.x / kXcds) >= each || tile >= all) return;
+  const int tm = tile / ntile_b, tb = tile - tm * ntile_b;
+  const int r0 = tm * 16 * WR, b0 = tb * 16 * NJ;
+  const int kp = p.kp;
+  const __amdgpu_buffer_rsrc_t rw = bounded_rsrc(p.w, static_cast<unsigned>(p.m) * p.k);
+  const int groups = row_groups(p.a.batch);
+  const __amdgpu_buffer_rsrc_t ra = bounded_rsrc(p.codes, static_cast<unsigned>(groups) * 16 * kp);
+  unsigned wo[WR], xo[NJ];
+#pragma unroll
+  for (int r = 0; r < WR; r++) wo[r] = r0 + 16 * r + ln < p.m ? static_cast<unsigned>(r0 + 16 * r + ln) * p.k + 16 * lg : kNoRec;
+#pragma unroll
+  for (int j = 0; j < NJ; j++) xo[j] = tb * NJ + j < groups ? static_cast<unsigned>(tb * NJ + j) * 1024 + 16 * lane : kNoRec;
+  const int steps = (p.k + 63) / 64, q = steps / KS, rem = steps % KS;
+  const int s0 = q * wave + min(wave, rem), s1 = s0 + q + (wave < rem ? 1 : 0);
+  i32x4 w[U][WR], x[U][NJ];
+  auto issue = [&](int u, int s) {  // past the last step: zeros
+    const bool ok = s < s1;
+#pragma unroll
+    for (int r = 0; r < WR; r++)
+      w[u][r] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rw, ok ? wo[r] : kNoRec, 64 * s, 0));
+    if constexpr (!kFused) {
+#pragma unroll
+      for (int j = 0; j < NJ; j++)
+        x[u][j] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(ra, ok ? xo[j] : kNoRec, s * groups * 1024, 0));
+    }
+  };
+  i32x4 acc[NB];
+#pragma unroll
+  for (int i = 0; i < NB; i++) acc[i] = i32x4{0, 0, 0, 0};
+#pragma unroll
+  for (int u = 0; u < U; u++) issue(u, s0 + u);
+  // the epilogue's scales of this lane's first block, in flight too
+  const int ob = b0 + 16 * (wave % NJ) + ln, orow = r0 + 16 * (wave / NJ) + 4 * lg;
+  Epi4 epi;
+  if (wave < NB) epi.load(p, ob, orow, !kFused);
+  if constexpr (kFused) {
+    for (int b = 0; b < p.a.batch; b++) {
+      const float s = quant_row<NV, 256, true>(p, b, tile == 0, red + 4 * (b & 1), [&](int i, uint32_t c) {
+        *reinterpret_cast<uint32_t *>(codes + b * kp + i) = c;
+      });
+      if (threadIdx.x == 0) made[b] = s;
+    }
+    __syncthreads();
+  }
+  for (int s = s0; s < s1; s += U) {
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if constexpr (kFused) x[u][0] = *reinterpret_cast<const i32x4 *>(codes + min(ln, p.a.batch - 1) * kp + min(64 * (s + u), kp - 64) + 16 * lg);
+#pragma unroll
+      for (int r = 0; r < WR; r++)
+#pragma unroll
+        for (int j = 0; j < NJ; j++)
+          acc[r * NJ + j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u][r], x[u][j], acc[r * NJ + j], 0, 0, 0);
+      issue(u, s + u + U);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NB; i++) *reinterpret_cast<i32x4 *>(&part[wave][i][4 * lane]) = acc[i];
+  __syncthreads();
+  for (int i = wave; i < NB; i += KS) {
+    i32x4 sum = *reinterpret_cast<const i32x4 *>(&part[0][i][4 * lane]);
+#pragma unroll
+    for (int k = 1; k < KS; k++) {
+      const i32x4 v = *reinterpret_cast<const i32x4 *>(&part[k][i][4 * lane]);
+#pragma unroll
+      for (int z = 0; z < 4; z++) sum[z] += v[z];
+    }
+    const int b = b0 + 16 * (i % NJ) + ln, r = r0 + 16 * (i / NJ) + 4 * lg;
+    if (i != wave) epi.load(p, b, r, !kFused);
+    if (kFused) epi.s = made[min(ln, p.a.batch - 1)];
+    if (b < p.a.batch && r < p.m) epi.finish(p, b, r, sum);
+  }
+}
+
+// Outputs of NR activation rows x 4 C weight rows whose sums lie in LDS, rows
+// of `stride`: lane l has weight rows r0 + 4 (l % C) .. + 3 of every (64 / C)th
+// activation row.  Four rows' residuals load together.
+template <int ACT, int C, int NR>
+__device__ __forceinline__ void rows_out(const RowsQ8 &p, const int *sums, int stride, int b0, int bj, int r0, const float *sc,
+                                         const f32x4 &ws, const f32x4 &bi) {
+  constexpr int RW = 64 / C, U = NR / RW < 4 ? NR / RW : 4;  // rows a wave has at once
+  const int lane = threadIdx.x & 63, c = 4 * (lane % C), r = r0 + c;
+  if (r >= p.m) return;
+  const int mo = ACT == XE_ACT_GEGLU ? p.m / 2 : p.m, ro = ACT == XE_ACT_GEGLU ? r / 2 : r;
+  constexpr int NO = ACT == XE_ACT_GEGLU ? 2 : 4;
+  typedef float OutV __attribute__((ext_vector_type(NO)));
+#pragma unroll 1
+  for (int i0 = lane / C; i0 < NR; i0 += U * RW) {
+    OutV e[U];
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (p.a.res) e[u] = *reinterpret_cast<const OutV *>(p.a.res + static_cast<size_t>(min(b0 + bj + i0 + u * RW, p.a.batch - 1)) * mo + ro);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int row = i0 + u * RW, b = b0 + bj + row;
+      if (b >= p.a.batch) continue;
+      const i32x4 v = *reinterpret_cast<const i32x4 *>(sums + row * stride + c);
+      const float s = sc[bj + row];
+      float z[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        z[i] = static_cast<float>(v[i]) * s * ws[i];
+        if (p.bias) z[i] += bi[i];
+      }
+      OutV y;
+#pragma unroll
+      for (int i = 0; i < NO; i++) y[i] = ACT == XE_ACT_GEGLU ? gelu_tanh_f(z[2 * i % 4]) * z[2 * i % 4 + 1] : activate(ACT, z[i]);
+      if (p.a.res)
+#pragma unroll
+        for (int i = 0; i < NO; i++) y[i] += e[u][i];
+      *reinterpret_cast<OutV *>(p.a.y + static_cast<size_t>(b) * mo + ro) = y;
+    }
+  }
+}
+
+// Tiles of BM weight rows x BN activation rows a workgroup, four waves of BM /
+// 2 x BN / 2; K in steps of 128 bytes through two LDS buffers, the loads of two
+// more steps in registers.  Rows lie 128 bytes apart in LDS, their 16-byte
+// chunks permuted by the row, so that 16 rows read together cover all banks.
+// Each tile begins at another step: rows K apart share an L2 channel where K is
+// a multiple of 4096, and the tiles that run at once then spread over them.
+template <int BM, int BN>
+__global__ __launch_bounds__(256, BM * BN <= 128 * 128 ? 2 : 1) void rows_tile_kernel(RowsQ8 p, int ntile_m, int ntile_b, int ksplit) {
+  constexpr int NA = BM / 32, NX = BN / 32;    // 16-byte chunks a thread loads of each operand
+  constexpr int FM = BM / 32, FN = BN / 32;    // 16 x 16 blocks of a wave
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2][(BM + BN) * kStep];
+  __shared__ float sc[BN];
+  __shared__ int flag;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int ln = lane & 15, lg = lane >> 4, wm = wave >> 1, wn = wave & 1;
+  const int all = ntile_m * ntile_b * ksplit, each = (all + kXcds - 1) / kXcds;
+  const int at = static_cast<int>(blockIdx.x % kXcds) * each + static_cast<int>(blockIdx.x / kXcds);
+  if (static_cast<int>(blockIdx.x / kXcds) >= each || at >= all) return;
+  const int tb = at % ntile_b, rest = at / ntile_b, z = rest % ksplit, tm = rest / ksplit;
+  const int m0 = tm * BM, b0 = tb * BN;
+  const __amdgpu_buffer_rsrc_t rw = bounded_rsrc(p.w, static_cast<unsigned>(p.m) * p.k);
+  const int groups = row_groups(p.a.batch);
+  const __amdgpu_buffer_rsrc_t ra = bounded_rsrc(p.codes, static_cast<unsigned>(groups) * 16 * p.kp);
+  const int steps = p.kp / kStep, q = steps / ksplit, rem = steps % ksplit;
+  const int s0 = q * z + min(z, rem), ns = q + (z < rem ? 1 : 0);
+#ifndef XE_RQ_ROT
+#define XE_RQ_ROT 5
+#endif
+  const int rot = (tm * XE_RQ_ROT) % max(ns, 1);
+  // thread t takes chunk t % 8 of weight rows t / 8 + 32 j; wave w the blocks w + 4 j
+  // of the activations, 64 k of the first 16 rows, of the second, ..
+  const int xc = tid & 7, xr = tid >> 3;
+  unsigned wo[NA], xo[NX];
+#pragma unroll
+  for (int j = 0; j < NA; j++) wo[j] = m0 + xr + 32 * j < p.m ? static_cast<unsigned>(m0 + xr + 32 * j) * p.k + 16 * xc : kNoRec;
+#pragma unroll
+  for (int j = 0; j < NX; j++) {
+    const int h = (wave + 4 * j) / (BN / 16), g = (wave + 4 * j) % (BN / 16);
+    xo[j] = b0 / 16 + g < groups ? static_cast<unsigned>(h * groups + b0 / 16 + g) * 1024 + 16 * lane : kNoRec;
+  }
+  struct Stage {
+    i32x4 w[NA], x[NX];
+  } st[2];
+  auto issue = [&](int i, Stage &g) {  // past the last step: zeros
+    int s = i + rot;
+    s = s0 + (s >= ns ? s - ns : s);
+    const bool ok = i < ns;
+#pragma unroll
+    for (int j = 0; j < NA; j++)
+      g.w[j] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rw, ok ? wo[j] : kNoRec, s * kStep, 0));
+#pragma unroll
+    for (int j = 0; j < NX; j++)
+      g.x[j] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(ra, ok ? xo[j] : kNoRec, s * 2 * groups * 1024, 0));
+  };
+  const int put_at = xr * kStep + ((xc ^ (xr & 7)) << 4);
+  auto put = [&](int buf, const Stage &g) {
+#pragma unroll
+    for (int j = 0; j < NA; j++) *reinterpret_cast<i32x4 *>(&lds[buf][put_at + 32 * j * kStep]) = g.w[j];
+#pragma unroll
+    for (int j = 0; j < NX; j++) {
+      const int h = (wave + 4 * j) / (BN / 16), rg = (wave + 4 * j) % (BN / 16);
+      *reinterpret_cast<i32x4 *>(&lds[buf][(BM + 16 * rg + ln) * kStep + (((4 * h + lg) ^ (ln & 7)) << 4)]) = g.x[j];
+    }
+  };
+  const int wbase = (wm * (BM / 2) + ln) * kStep, xbase = BM * kStep + (wn * (BN / 2) + ln) * kStep;
+  i32x4 acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; i++)
+#pragma unroll
+    for (int j = 0; j < FN; j++) acc[i][j] = i32x4{0, 0, 0, 0};
+  // A step's LDS reads, MFMAs, LDS writes of the next step and loads of the one
+  // after the next but one, spread over each other.
+  auto step = [&](int buf, int next) {
+    constexpr int R = FM + FN, M = FM * FN / R;
+    i32x4 w[2][FM], x[2][FN];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int c = ((4 * h + lg) ^ (ln & 7)) << 4;
+#pragma unroll
+      for (int i = 0; i < FM; i++) w[h][i] = *reinterpret_cast<const i32x4 *>(&lds[buf][wbase + 16 * i * kStep + c]);
+#pragma unroll
+      for (int j = 0; j < FN; j++) x[h][j] = *reinterpret_cast<const i32x4 *>(&lds[buf][xbase + 16 * j * kStep + c]);
+    }
+    put(buf ^ 1, st[buf ^ 1]);
+    issue(next, st[buf ^ 1]);
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int i = 0; i < FM; i++)
+#pragma unroll
+        for (int j = 0; j < FN; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[h][i], x[h][j], acc[i][j], 0, 0, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+      __builtin_amdgcn_sched_group_barrier(0x8, M, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+      __builtin_amdgcn_sched_group_barrier(0x8, M, 0);
+      __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);
+    }
+    __syncthreads();
+  };
+  issue(0, st[0]);
+  issue(1, st[1]);
+  // the epilogue's scales: of the tile's activation rows, of a lane's weight rows
+  for (int i = tid; i < BN; i += 256) sc[i] = b0 + i < p.a.batch ? p.scales[b0 + i] : 0.f;
+  f32x4 ws4 = {0.f, 0.f, 0.f, 0.f}, bi4 = ws4;
+  {
+    const int r = m0 + wm * (BM / 2) + 4 * (lane % (BM / 8));
+    if (p.vec && r < p.m) {
+      ws4 = *reinterpret_cast<const f32x4 *>(p.ws + r);
+      if (p.bias) bi4 = *reinterpret_cast<const f32x4 *>(p.bias + r);
+    }
+  }
+  put(0, st[0]);
+  issue(2, st[0]);
+  __syncthreads();
+  int i = 0;
+  for (; i + 2 <= ns; i += 2) {
+    step(0, i + 3);
+    step(1, i + 4);
+  }
+  if (i < ns) step(0, i + 3);
+  if (ksplit > 1) {
+    constexpr int W4 = BM * BN / 4;  // i32x4 of a tile
+    const size_t tile = static_cast<size_t>(tm) * ntile_b + tb;
+    const __amdgpu_buffer_rsrc_t rp = gdev::coherent_rsrc(reinterpret_cast<const i32x4 *>(p.part) + tile * ksplit * W4);
+#pragma unroll
+    for (int i = 0; i < FM; i++)
+#pragma unroll
+      for (int j = 0; j < FN; j++)
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc[i][j]), rp,
+                                               static_cast<int>((z * W4 + (i * FN + j) * 256 + tid) * 16), 0, gdev::kCoherentSc1);
+    if (!adev::last_to_arrive(p.cnt + tile, ksplit, &flag)) return;
+    if (tid == 0) __hip_atomic_store(p.cnt + tile, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int o = 0; o < ksplit; o++) {
+      if (o == z) continue;
+#pragma unroll
+      for (int i = 0; i < FM; i++)
+#pragma unroll
+        for (int j = 0; j < FN; j++) {
+          const i32x4 v = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(
+              rp, static_cast<int>((o * W4 + (i * FN + j) * 256 + tid) * 16), 0, gdev::kCoherentSc1));
+#pragma unroll
+          for (int e = 0; e < 4; e++) acc[i][j][e] += v[e];
+        }
+    }
+  }
+  // Sums turn through the wave's part of LDS, so that a row's outputs go out
+  // side by side: a lane always has the same four weight rows.
+  constexpr int RS = BM / 2 + 4, JH = FN > 1 ? 2 : 1;  // 16 JH activation rows at a time
+  static_assert(4 * 16 * JH * RS * 4 <= sizeof(lds), "the waves' rows fit the operand buffers");
+  int *const out = reinterpret_cast<int *>(&lds[0][0]) + wave * 16 * JH * RS;
+#pragma unroll
+  for (int j0 = 0; j0 < FN; j0 += JH) {
+#pragma unroll
+    for (int j = 0; j < JH; j++)
+#pragma unroll
+      for (int i = 0; i < FM; i++) *reinterpret_cast<i32x4 *>(out + (16 * j + ln) * RS + 16 * i + 4 * lg) = acc[i][j0 + j];
+    __builtin_amdgcn_wave_barrier();
+    const int bj = wn * (BN / 2) + 16 * j0, rj = m0 + wm * (BM / 2);
+    if (p.vec) {
+      switch (p.a.act) {
+        case XE_ACT_RELU: rows_out<XE_ACT_RELU, BM / 8, 16 * JH>(p, out, RS, b0, bj, rj, sc, ws4, bi4); break;
+        case XE_ACT_GELU: rows_out<XE_ACT_GELU, BM / 8, 16 * JH>(p, out, RS, b0, bj, rj, sc, ws4, bi4); break;
+        case XE_ACT_SILU: rows_out<XE_ACT_SILU, BM / 8, 16 * JH>(p, out, RS, b0, bj, rj, sc, ws4, bi4); break;
+        case XE_ACT_GEGLU: rows_out<XE_ACT_GEGLU, BM / 8, 16 * JH>(p, out, RS, b0, bj, rj, sc, ws4, bi4); break;
+        default: rows_out<XE_ACT_NONE, BM / 8, 16 * JH>(p, out, RS, b0, bj, rj, sc, ws4, bi4);
+      }
+    } else {
+#pragma unroll 1
+      for (int id = lane; id < 16 * JH * (BM / 8); id += 64) {
+        const int row = id / (BM / 8), c = 4 * (id % (BM / 8));
+        if (b0 + bj + row >= p.a.batch || rj + c >= p.m) continue;
+        Epi4 epi;
+        epi.load(p, b0 + bj + row, rj + c, true);
+        epi.finish(p, b0 + bj + row, rj + c, *reinterpret_cast<const i32x4 *>(out + row * RS + c));
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+template <int WR, int NJ, int KS, int U, int NV = 0>
+void launch_gemm(const RowsQ8 &r, hipStream_t s) {
+  const int tm = (r.m + 16 * WR - 1) / (16 * WR), tb = (r.a.batch + 16 * NJ - 1) / (16 * NJ);
+  const int blocks = (tm * tb + kXcds - 1) / kXcds * kXcds;
+  hipLaunchKernelGGL((rows_gemm_kernel<WR, NJ, KS, U, NV>), dim3(blocks), dim3(64 * KS), 0, s, r, tm, tb);
+  XE_HIP(hipGetLastError());
+}
+
+template <int BM, int BN>
+void launch_tile(const RowsQ8 &r, int ksplit, hipStream_t s) {
+  const int tm = (r.m + BM - 1) / BM, tb = (r.a.batch + BN - 1) / BN;
+  // the partial tiles and their counters fit the workspace, or K is not split
+  if (static_cast<size_t>(tm) * tb > kCntWords || static_cast<size_t>(tm) * tb * ksplit * BM * BN * 4 > kPartBytes) ksplit = 1;
+  const int blocks = (tm * tb * ksplit + kXcds - 1) / kXcds * kXcds;
+  hipLaunchKernelGGL((rows_tile_kernel<BM, BN>), dim3(blocks), dim3(256), 0, s, r, tm, tb, ksplit);
+  XE_HIP(hipGetLastError());
+}
+
+// Whether what one workgroup writes may be what another still reads, were rows
+// quantised and products finished in one launch.
+bool shares(const RowsQ8 &r, int outs) {
+  const size_t in = static_cast<size_t>(r.a.batch) * r.k * 4, out = static_cast<size_t>(r.a.batch) * outs * 4;
+  auto meet = [](const float *a, size_t n, const float *b, size_t m) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a && b && x < y + m && y < x + n;
+  };
+  return meet(r.a.sum, in, r.a.x, in) || meet(r.a.sum, in, r.a.add, in) || meet(r.a.sum, in, r.a.res, out) || meet(r.a.sum, in, r.a.y, out) ||
+         meet(r.a.y, out, r.a.x, in) || meet(r.a.y, out, r.a.add, in);
+}
+
+template <bool VEC>
+void launch_quant(const RowsQ8 &r, hipStream_t s) {
+  const dim3 rows(r.a.batch);
+  if (r.k <= 1024) hipLaunchKernelGGL((rows_quant_kernel<1, 256, VEC>), rows, dim3(256), 0, s, r);
+  else if (r.k <= 2048) hipLaunchKernelGGL((rows_quant_kernel<2, 256, VEC>), rows, dim3(256), 0, s, r);
+  else if (r.k <= 4096) hipLaunchKernelGGL((rows_quant_kernel<4, 256, VEC>), rows, dim3(256), 0, s, r);
+  else if (r.k <= 8192) hipLaunchKernelGGL((rows_quant_kernel<4, 512, VEC>), rows, dim3(512), 0, s, r);
+  else if (r.k <= 16384) hipLaunchKernelGGL((rows_quant_kernel<4, 1024, VEC>), rows, dim3(1024), 0, s, r);
+  else hipLaunchKernelGGL((rows_quant_kernel<8, 1024, VEC>), rows, dim3(1024), 0, s, r);
+  XE_HIP(hipGetLastError());
 }
 
 }  // namespace
 
-void launch_rows_q8(const RowsQ8 &r, hipStream_t s) {
-  const dim3 rows(r.a.batch);
-  if (r.k <= 2048) hipLaunchKernelGGL((rows_quant_kernel<8, 256>), rows, dim3(256), 0, s, r);
-  else if (r.k <= 8192) hipLaunchKernelGGL((rows_quant_kernel<16, 512>), rows, dim3(512), 0, s, r);
-  else hipLaunchKernelGGL((rows_quant_kernel<32, 1024>), rows, dim3(1024), 0, s, r);
-  XE_HIP(hipGetLastError());
-  hipLaunchKernelGGL(rows_gemm_kernel, dim3((r.m + 63) / 64, (r.a.batch + 15) / 16), dim3(kT), 0, s, r);
-  XE_HIP(hipGetLastError());
+size_t rows_q8_ws_bytes() { return 2048 + kCntWords * 4 + kPartBytes; }
+
+size_t rows_q8_codes_bytes(int batch, int k) { return static_cast<size_t>(row_groups(batch)) * 16 * ((k + kStep - 1) / kStep * kStep); }
+
+void launch_rows_q8(const RowsQ8 &L, hipStream_t s) {
+  RowsQ8 r = L;
+  r.kp = (r.k + kStep - 1) / kStep * kStep;
+  const int outs = r.a.act == XE_ACT_GEGLU ? r.m / 2 : r.m;
+  r.vec = outs % 4 == 0 && ((reinterpret_cast<uintptr_t>(r.a.y) | reinterpret_cast<uintptr_t>(r.a.res) |
+                             reinterpret_cast<uintptr_t>(r.ws) | reinterpret_cast<uintptr_t>(r.bias)) & 15) == 0;
+  const bool in16 = ((reinterpret_cast<uintptr_t>(r.a.x) | reinterpret_cast<uintptr_t>(r.a.add) | reinterpret_cast<uintptr_t>(r.a.sum) |
+                      reinterpret_cast<uintptr_t>(r.a.post_w)) & 15) == 0;
+#ifndef XE_RQ_FW
+#define XE_RQ_FW 1, 1, 4, 8
+#endif
+#ifndef XE_RQ_FUSE
+#define XE_RQ_FUSE 1
+#endif
+  if (XE_RQ_FUSE && in16 && r.k <= 4096 && r.a.batch <= 16 && r.a.batch * r.kp <= kFusedBytes && !shares(r, outs)) {
+    if (r.k <= 1024) launch_gemm<XE_RQ_FW, 1>(r, s);
+    else if (r.k <= 2048) launch_gemm<XE_RQ_FW, 2>(r, s);
+    else launch_gemm<XE_RQ_FW, 4>(r, s);
+    return;
+  }
+  if (in16) launch_quant<true>(r, s);
+  else launch_quant<false>(r, s);
+#ifndef XE_RQ_V
+#define XE_RQ_V 0
+#endif
+  switch (XE_RQ_V) {
+    case 1: launch_gemm<1, 1, 4, 8>(r, s); return;
+    case 2: launch_gemm<1, 1, 8, 4>(r, s); return;
+    case 3: launch_gemm<1, 2, 4, 4>(r, s); return;
+    case 4: launch_gemm<1, 4, 4, 4>(r, s); return;
+    case 5: launch_gemm<1, 4, 8, 4>(r, s); return;
+    case 6: launch_gemm<2, 4, 4, 3>(r, s); return;
+    case 7: launch_gemm<4, 4, 4, 3>(r, s); return;
+    case 8: launch_gemm<4, 4, 4, 2>(r, s); return;
+    case 9: launch_gemm<8, 4, 4, 2>(r, s); return;
+    case 10: launch_gemm<4, 8, 4, 2>(r, s); return;
+    case 11: launch_gemm<2, 2, 4, 4>(r, s); return;
+    case 12: launch_gemm<8, 2, 4, 2>(r, s); return;
+    case 13: launch_gemm<2, 4, 8, 3>(r, s); return;
+    case 14: launch_gemm<4, 2, 4, 3>(r, s); return;
+    case 15: launch_gemm<2, 1, 4, 6>(r, s); return;
+    case 16: launch_gemm<2, 2, 8, 3>(r, s); return;
+    case 17: launch_gemm<4, 1, 4, 4>(r, s); return;
+    case 18: launch_gemm<1, 2, 8, 4>(r, s); return;
+    case 21: launch_tile<256, 128>(r, 1, s); return;
+    case 22: launch_tile<256, 128>(r, 2, s); return;
+    case 23: launch_tile<128, 128>(r, 1, s); return;
+    case 24: launch_tile<128, 128>(r, 2, s); return;
+    case 25: launch_tile<128, 128>(r, 4, s); return;
+    case 26: launch_tile<128, 64>(r, 1, s); return;
+    case 27: launch_tile<128, 64>(r, 2, s); return;
+    case 28: launch_tile<64, 64>(r, 1, s); return;
+    case 29: launch_tile<64, 64>(r, 2, s); return;
+    case 30: launch_tile<64, 64>(r, 4, s); return;
+    case 31: launch_tile<64, 128>(r, 1, s); return;
+    case 32: launch_tile<64, 128>(r, 2, s); return;
+  }
+  launch_gemm<1, 4, 4, 4>(r, s);
 }
 
 }  // namespace xe
