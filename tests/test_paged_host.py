@@ -159,6 +159,42 @@ int main() {
     subprocess.check_call([exe], timeout=60)
 
 
+def test_forms_of_the_rows_product(tmp_path):
+    """Every form is taken by some shape, by one of those that the GPU tests run
+    among them, and none whose partial tiles do not fit the workspace."""
+    if shutil.which("g++") is None:
+        pytest.skip("no g++")
+    src = tmp_path / "f.cpp"
+    src.write_text(r'''
+#include "rows_form.h"
+#include <cassert>
+#include <initializer_list>
+using namespace xe::rowsform;
+int main() {
+  int seen[kForms] = {};
+  for (int m : {1, 15, 16, 100, 1000, 4096, 14336, 65536, 1000000, 134217727})
+    for (int k : {16, 64, 1152, 4096, 16384, 32768})
+      for (int batch : {1, 2, 3, 16, 33, 64, 65, 200, 511, 512})
+        for (int cus : {1, 64, 256, 304}) {
+          const int i = pick(m, k, batch, cus);
+          assert(i >= 0 && i < kForms && fits(i, m, batch));
+        }
+  for (int i = 0; i < kForms; i++)
+    if (kForm[i].ksplit > 1 && i >= kInWaves) {
+      assert(fits(i, kForm[i].bm, kForm[i].bn) && !fits(i, 134217727, 512));
+      assert(!fits(i, kForm[i].bm * (kTiles + 1), 1));
+    }
+  const int tests[][3] = {{200, 192, 3},     {200, 192, 512},   {301, 720, 509},  {702, 160, 511},   {702, 4112, 397},
+                          {702, 8208, 197}, {2102, 304, 509}, {4102, 1040, 510}, {8200, 8208, 449}};
+  for (auto &t : tests) seen[pick(t[0], t[1], t[2], 256)]++;
+  for (int n : seen) assert(n == 1);
+}
+''')
+    exe = str(tmp_path / "f")
+    subprocess.check_call(["g++", "-O1", "-std=c++17", "-fsanitize=undefined,address", "-I" + CSRC, str(src), "-o", exe])
+    subprocess.check_call([exe], timeout=60)
+
+
 def fails(xe, call, *args):
     assert call(None, *args) == -1
     return xe.last_error()

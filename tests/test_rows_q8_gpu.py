@@ -68,6 +68,15 @@ def test_shapes(gpu, xe, m, k, batch):
     rows_case(xe, gpu, m, k, batch, norm=1, seed=5)
 
 
+@pytest.mark.parametrize("m,k,batch", [(301, 720, 509), (702, 160, 511), (702, 4112, 397), (702, 8208, 197), (2102, 304, 509),
+                                       (4102, 1040, 510), (8200, 8208, 449)])
+@pytest.mark.parametrize("act", [1, 4])
+def test_larger_shapes(gpu, xe, m, k, batch, act):
+    """Every form of the product, with tiles that end outside in both directions."""
+    m += m % 2 if act == 4 else 0
+    rows_case(xe, gpu, m, k, batch, norm=2, act=act, res=True, want_sum=False, seed=2)
+
+
 @pytest.mark.parametrize("act", [0, 1, 2, 3, 4])
 @pytest.mark.parametrize("batch", [1, 7, 30, 130])
 @pytest.mark.parametrize("bias,res", [(True, True), (False, False)])

@@ -1163,8 +1163,7 @@ int xe_w8a8_rows_dev(xe_ctx *ctx, const xe_weight *w, const xe_w8a8_rows *rows) 
     r.cnt = reinterpret_cast<unsigned *>(ctx->rows_ws + 2048);
     r.part = reinterpret_cast<int *>(ctx->rows_ws + kRowsPart);
     r.codes = reinterpret_cast<int8_t *>(ctx->rows_codes);
-    launch_rows_q8(r, ctx->dev->stream);
-    ctx->dispatches += 2;
+    ctx->dispatches += launch_rows_q8(r, ctx->dev->stream);
     return 0;
   }, -1);
 }

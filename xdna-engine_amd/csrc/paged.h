@@ -57,6 +57,6 @@ size_t rows_q8_codes_bytes(int batch, int k);
 // Scales (2 KB), then arrival counters (4 KB, zeroed once; they re-arm), then
 // partial tiles of K splits.
 size_t rows_q8_ws_bytes();
-void launch_rows_q8(const RowsQ8 &r, hipStream_t s);
+int launch_rows_q8(const RowsQ8 &r, hipStream_t s);  // returns its launches
 
 }  // namespace xe

@@ -8,18 +8,18 @@
 // not depend on the order of a sum: q and s are those of h itself.
 #include "attn_dev.h"
 #include "paged.h"
+#include "rows_form.h"
 
 namespace xe {
 namespace {
 
-constexpr int kT = 256;
 constexpr unsigned kNoRec = 0x7ffffff0u;  // past every buffer: loads return zeros
 
 constexpr int kXcds = 8;
-constexpr size_t kPartBytes = size_t(32) << 20;  // partial tiles of K splits
-constexpr size_t kCntWords = 1024;               // and their arrival counters
+constexpr size_t kPartBytes = rowsform::kPartBytes;  // partial tiles of K splits
+constexpr size_t kCntWords = rowsform::kTiles;       // and their arrival counters
 constexpr int kStep = 128;          // bytes of K a step
-constexpr int kFusedBytes = 8192;   // codes that a workgroup makes itself
+constexpr int kFusedK = 4096;       // K up to which a workgroup makes one row's codes itself
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
@@ -289,16 +289,15 @@ struct Epi4 {
 // waves each over their own part of K (v_mfma_i32_16x16x64_i8: a lane holds 16
 // consecutive k of weight row lane % 16 and of activation row lane % 16), U
 // steps of 64 in flight.  NV > 0: the workgroup makes the codes itself (K <= 1024
-// NV), into LDS, while its first weights load.
+// NV, one row), into LDS, while its first weights load.
 template <int WR, int NJ, int KS, int U, int NV>
 __global__ __launch_bounds__(64 * KS) void rows_gemm_kernel(RowsQ8 p, int ntile_m, int ntile_b) {
   constexpr int NB = WR * NJ;                     // 16 x 16 blocks
   constexpr bool kFused = NV > 0;
-  static_assert(!kFused || (KS == 4 && NJ == 1), "rows made here: 256 threads, 16 rows at most");
+  static_assert(!kFused || (KS == 4 && NJ == 1), "one row made here by 256 threads");
   __shared__ __attribute__((aligned(16))) int part[KS][NB][256];
-  __shared__ __attribute__((aligned(16))) int8_t codes[kFused ? kFusedBytes : 16];
-  __shared__ double red[kFused ? 8 : 1][4];
-  __shared__ float made[16];
+  __shared__ __attribute__((aligned(16))) int8_t codes[kFused ? kFusedK : 16];
+  __shared__ double red[kFused ? 4 : 1][4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 15, lg = lane >> 4;
   // The tiles of an XCD lie in a row, those of the same weight rows next to
@@ -341,18 +340,13 @@ __global__ __launch_bounds__(64 * KS) void rows_gemm_kernel(RowsQ8 p, int ntile_
   Epi4 epi;
   if (wave < NB) epi.load(p, ob, orow, !kFused);
   if constexpr (kFused) {
-    for (int b = 0; b < p.a.batch; b++) {
-      const float s = quant_row<NV, 256, true>(p, b, tile == 0, red + 4 * (b & 1), [&](int i, uint32_t c) {
-        *reinterpret_cast<uint32_t *>(codes + b * kp + i) = c;
-      });
-      if (threadIdx.x == 0) made[b] = s;
-    }
+    epi.s = quant_row<NV, 256, true>(p, 0, tile == 0, red, [&](int i, uint32_t c) { *reinterpret_cast<uint32_t *>(codes + i) = c; });
     __syncthreads();
   }
   for (int s = s0; s < s1; s += U) {
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      if constexpr (kFused) x[u][0] = *reinterpret_cast<const i32x4 *>(codes + min(ln, p.a.batch - 1) * kp + min(64 * (s + u), kp - 64) + 16 * lg);
+      if constexpr (kFused) x[u][0] = *reinterpret_cast<const i32x4 *>(codes + min(64 * (s + u), kp - 64) + 16 * lg);
 #pragma unroll
       for (int r = 0; r < WR; r++)
 #pragma unroll
@@ -374,7 +368,6 @@ __global__ __launch_bounds__(64 * KS) void rows_gemm_kernel(RowsQ8 p, int ntile_
     }
     const int b = b0 + 16 * (i % NJ) + ln, r = r0 + 16 * (i / NJ) + 4 * lg;
     if (i != wave) epi.load(p, b, r, !kFused);
-    if (kFused) epi.s = made[min(ln, p.a.batch - 1)];
     if (b < p.a.batch && r < p.m) epi.finish(p, b, r, sum);
   }
 }
@@ -420,16 +413,15 @@ __device__ __forceinline__ void rows_out(const RowsQ8 &p, const int *sums, int s
   }
 }
 
-// Tiles of BM weight rows x BN activation rows a workgroup, four waves of BM /
-// 2 x BN / 2; K in steps of 128 bytes through two LDS buffers, the loads of two
+// Tiles of BM weight rows x BN activation rows a workgroup, WV waves of 2 BM / WV
+// x BN / 2; K in steps of 128 bytes through two LDS buffers, the loads of two
 // more steps in registers.  Rows lie 128 bytes apart in LDS, their 16-byte
 // chunks permuted by the row, so that 16 rows read together cover all banks.
-// Each tile begins at another step: rows K apart share an L2 channel where K is
-// a multiple of 4096, and the tiles that run at once then spread over them.
-template <int BM, int BN>
-__global__ __launch_bounds__(256, BM * BN <= 128 * 128 ? 2 : 1) void rows_tile_kernel(RowsQ8 p, int ntile_m, int ntile_b, int ksplit) {
-  constexpr int NA = BM / 32, NX = BN / 32;    // 16-byte chunks a thread loads of each operand
-  constexpr int FM = BM / 32, FN = BN / 32;    // 16 x 16 blocks of a wave
+template <int BM, int BN, int WV>
+__global__ __launch_bounds__(64 * WV, 2) void rows_tile_kernel(RowsQ8 p, int ntile_m, int ntile_b, int ksplit) {
+  constexpr int T = 64 * WV, MW = BM / (WV / 2), NW = BN / 2;  // a wave's rows of weights, of activations
+  constexpr int NA = BM * 8 / T, NX = BN * 8 / T;              // 16-byte chunks a thread loads of each operand
+  constexpr int FM = MW / 16, FN = NW / 16;                    // 16 x 16 blocks of a wave
   __shared__ __attribute__((aligned(16))) uint8_t lds[2][(BM + BN) * kStep];
   __shared__ float sc[BN];
   __shared__ int flag;
@@ -445,27 +437,22 @@ __global__ __launch_bounds__(256, BM * BN <= 128 * 128 ? 2 : 1) void rows_tile_k
   const __amdgpu_buffer_rsrc_t ra = bounded_rsrc(p.codes, static_cast<unsigned>(groups) * 16 * p.kp);
   const int steps = p.kp / kStep, q = steps / ksplit, rem = steps % ksplit;
   const int s0 = q * z + min(z, rem), ns = q + (z < rem ? 1 : 0);
-#ifndef XE_RQ_ROT
-#define XE_RQ_ROT 5
-#endif
-  const int rot = (tm * XE_RQ_ROT) % max(ns, 1);
-  // thread t takes chunk t % 8 of weight rows t / 8 + 32 j; wave w the blocks w + 4 j
+  // thread t takes chunk t % 8 of weight rows t / 8 + T / 8 j; wave w the blocks w + WV j
   // of the activations, 64 k of the first 16 rows, of the second, ..
   const int xc = tid & 7, xr = tid >> 3;
   unsigned wo[NA], xo[NX];
 #pragma unroll
-  for (int j = 0; j < NA; j++) wo[j] = m0 + xr + 32 * j < p.m ? static_cast<unsigned>(m0 + xr + 32 * j) * p.k + 16 * xc : kNoRec;
+  for (int j = 0; j < NA; j++) wo[j] = m0 + xr + T / 8 * j < p.m ? static_cast<unsigned>(m0 + xr + T / 8 * j) * p.k + 16 * xc : kNoRec;
 #pragma unroll
   for (int j = 0; j < NX; j++) {
-    const int h = (wave + 4 * j) / (BN / 16), g = (wave + 4 * j) % (BN / 16);
+    const int h = (wave + WV * j) / (BN / 16), g = (wave + WV * j) % (BN / 16);
     xo[j] = b0 / 16 + g < groups ? static_cast<unsigned>(h * groups + b0 / 16 + g) * 1024 + 16 * lane : kNoRec;
   }
   struct Stage {
     i32x4 w[NA], x[NX];
   } st[2];
   auto issue = [&](int i, Stage &g) {  // past the last step: zeros
-    int s = i + rot;
-    s = s0 + (s >= ns ? s - ns : s);
+    const int s = s0 + i;
     const bool ok = i < ns;
 #pragma unroll
     for (int j = 0; j < NA; j++)
@@ -477,14 +464,14 @@ __global__ __launch_bounds__(256, BM * BN <= 128 * 128 ? 2 : 1) void rows_tile_k
   const int put_at = xr * kStep + ((xc ^ (xr & 7)) << 4);
   auto put = [&](int buf, const Stage &g) {
 #pragma unroll
-    for (int j = 0; j < NA; j++) *reinterpret_cast<i32x4 *>(&lds[buf][put_at + 32 * j * kStep]) = g.w[j];
+    for (int j = 0; j < NA; j++) *reinterpret_cast<i32x4 *>(&lds[buf][put_at + T / 8 * j * kStep]) = g.w[j];
 #pragma unroll
     for (int j = 0; j < NX; j++) {
-      const int h = (wave + 4 * j) / (BN / 16), rg = (wave + 4 * j) % (BN / 16);
+      const int h = (wave + WV * j) / (BN / 16), rg = (wave + WV * j) % (BN / 16);
       *reinterpret_cast<i32x4 *>(&lds[buf][(BM + 16 * rg + ln) * kStep + (((4 * h + lg) ^ (ln & 7)) << 4)]) = g.x[j];
     }
   };
-  const int wbase = (wm * (BM / 2) + ln) * kStep, xbase = BM * kStep + (wn * (BN / 2) + ln) * kStep;
+  const int wbase = (wm * MW + ln) * kStep, xbase = BM * kStep + (wn * NW + ln) * kStep;
   i32x4 acc[FM][FN];
 #pragma unroll
   for (int i = 0; i < FM; i++)
@@ -493,7 +480,7 @@ __global__ __launch_bounds__(256, BM * BN <= 128 * 128 ? 2 : 1) void rows_tile_k
   // A step's LDS reads, MFMAs, LDS writes of the next step and loads of the one
   // after the next but one, spread over each other.
   auto step = [&](int buf, int next) {
-    constexpr int R = FM + FN, M = FM * FN / R;
+    constexpr int R = FM + FN, M = FM * FN / R, P = NA + NX;
     i32x4 w[2][FM], x[2][FN];
 #pragma unroll
     for (int h = 0; h < 2; h++) {
@@ -518,8 +505,8 @@ __global__ __launch_bounds__(256, BM * BN <= 128 * 128 ? 2 : 1) void rows_tile_k
       __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
 #pragma unroll
-    for (int i = 0; i < R; i++) {
-      __builtin_amdgcn_sched_group_barrier(0x8, M, 0);
+    for (int i = 0; i < P; i++) {
+      __builtin_amdgcn_sched_group_barrier(0x8, FM * FN / P, 0);
       __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
       __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);
     }
@@ -528,10 +515,10 @@ __global__ __launch_bounds__(256, BM * BN <= 128 * 128 ? 2 : 1) void rows_tile_k
   issue(0, st[0]);
   issue(1, st[1]);
   // the epilogue's scales: of the tile's activation rows, of a lane's weight rows
-  for (int i = tid; i < BN; i += 256) sc[i] = b0 + i < p.a.batch ? p.scales[b0 + i] : 0.f;
+  for (int i = tid; i < BN; i += T) sc[i] = b0 + i < p.a.batch ? p.scales[b0 + i] : 0.f;
   f32x4 ws4 = {0.f, 0.f, 0.f, 0.f}, bi4 = ws4;
   {
-    const int r = m0 + wm * (BM / 2) + 4 * (lane % (BM / 8));
+    const int r = m0 + wm * MW + 4 * (lane % (MW / 4));
     if (p.vec && r < p.m) {
       ws4 = *reinterpret_cast<const f32x4 *>(p.ws + r);
       if (p.bias) bi4 = *reinterpret_cast<const f32x4 *>(p.bias + r);
@@ -555,7 +542,7 @@ __global__ __launch_bounds__(256, BM * BN <= 128 * 128 ? 2 : 1) void rows_tile_k
 #pragma unroll
       for (int j = 0; j < FN; j++)
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc[i][j]), rp,
-                                               static_cast<int>((z * W4 + (i * FN + j) * 256 + tid) * 16), 0, gdev::kCoherentSc1);
+                                               static_cast<int>((z * W4 + (i * FN + j) * T + tid) * 16), 0, gdev::kCoherentSc1);
     if (!adev::last_to_arrive(p.cnt + tile, ksplit, &flag)) return;
     if (tid == 0) __hip_atomic_store(p.cnt + tile, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     for (int o = 0; o < ksplit; o++) {
@@ -565,7 +552,7 @@ __global__ __launch_bounds__(256, BM * BN <= 128 * 128 ? 2 : 1) void rows_tile_k
 #pragma unroll
         for (int j = 0; j < FN; j++) {
           const i32x4 v = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(
-              rp, static_cast<int>((o * W4 + (i * FN + j) * 256 + tid) * 16), 0, gdev::kCoherentSc1));
+              rp, static_cast<int>((o * W4 + (i * FN + j) * T + tid) * 16), 0, gdev::kCoherentSc1));
 #pragma unroll
           for (int e = 0; e < 4; e++) acc[i][j][e] += v[e];
         }
@@ -573,8 +560,8 @@ __global__ __launch_bounds__(256, BM * BN <= 128 * 128 ? 2 : 1) void rows_tile_k
   }
   // Sums turn through the wave's part of LDS, so that a row's outputs go out
   // side by side: a lane always has the same four weight rows.
-  constexpr int RS = BM / 2 + 4, JH = FN > 1 ? 2 : 1;  // 16 JH activation rows at a time
-  static_assert(4 * 16 * JH * RS * 4 <= sizeof(lds), "the waves' rows fit the operand buffers");
+  constexpr int RS = MW + 4, JH = FN > 1 ? 2 : 1;  // 16 JH activation rows at a time
+  static_assert(WV * 16 * JH * RS * 4 <= sizeof(lds), "the waves' rows fit the operand buffers");
   int *const out = reinterpret_cast<int *>(&lds[0][0]) + wave * 16 * JH * RS;
 #pragma unroll
   for (int j0 = 0; j0 < FN; j0 += JH) {
@@ -583,19 +570,19 @@ __global__ __launch_bounds__(256, BM * BN <= 128 * 128 ? 2 : 1) void rows_tile_k
 #pragma unroll
       for (int i = 0; i < FM; i++) *reinterpret_cast<i32x4 *>(out + (16 * j + ln) * RS + 16 * i + 4 * lg) = acc[i][j0 + j];
     __builtin_amdgcn_wave_barrier();
-    const int bj = wn * (BN / 2) + 16 * j0, rj = m0 + wm * (BM / 2);
+    const int bj = wn * NW + 16 * j0, rj = m0 + wm * MW;
     if (p.vec) {
       switch (p.a.act) {
-        case XE_ACT_RELU: rows_out<XE_ACT_RELU, BM / 8, 16 * JH>(p, out, RS, b0, bj, rj, sc, ws4, bi4); break;
-        case XE_ACT_GELU: rows_out<XE_ACT_GELU, BM / 8, 16 * JH>(p, out, RS, b0, bj, rj, sc, ws4, bi4); break;
-        case XE_ACT_SILU: rows_out<XE_ACT_SILU, BM / 8, 16 * JH>(p, out, RS, b0, bj, rj, sc, ws4, bi4); break;
-        case XE_ACT_GEGLU: rows_out<XE_ACT_GEGLU, BM / 8, 16 * JH>(p, out, RS, b0, bj, rj, sc, ws4, bi4); break;
-        default: rows_out<XE_ACT_NONE, BM / 8, 16 * JH>(p, out, RS, b0, bj, rj, sc, ws4, bi4);
+        case XE_ACT_RELU: rows_out<XE_ACT_RELU, MW / 4, 16 * JH>(p, out, RS, b0, bj, rj, sc, ws4, bi4); break;
+        case XE_ACT_GELU: rows_out<XE_ACT_GELU, MW / 4, 16 * JH>(p, out, RS, b0, bj, rj, sc, ws4, bi4); break;
+        case XE_ACT_SILU: rows_out<XE_ACT_SILU, MW / 4, 16 * JH>(p, out, RS, b0, bj, rj, sc, ws4, bi4); break;
+        case XE_ACT_GEGLU: rows_out<XE_ACT_GEGLU, MW / 4, 16 * JH>(p, out, RS, b0, bj, rj, sc, ws4, bi4); break;
+        default: rows_out<XE_ACT_NONE, MW / 4, 16 * JH>(p, out, RS, b0, bj, rj, sc, ws4, bi4);
       }
     } else {
 #pragma unroll 1
-      for (int id = lane; id < 16 * JH * (BM / 8); id += 64) {
-        const int row = id / (BM / 8), c = 4 * (id % (BM / 8));
+      for (int id = lane; id < 16 * JH * (MW / 4); id += 64) {
+        const int row = id / (MW / 4), c = 4 * (id % (MW / 4));
         if (b0 + bj + row >= p.a.batch || rj + c >= p.m) continue;
         Epi4 epi;
         epi.load(p, b0 + bj + row, rj + c, true);
@@ -614,13 +601,14 @@ void launch_gemm(const RowsQ8 &r, hipStream_t s) {
   XE_HIP(hipGetLastError());
 }
 
-template <int BM, int BN>
+template <int BM, int BN, int WV>
 void launch_tile(const RowsQ8 &r, int ksplit, hipStream_t s) {
   const int tm = (r.m + BM - 1) / BM, tb = (r.a.batch + BN - 1) / BN;
-  // the partial tiles and their counters fit the workspace, or K is not split
-  if (static_cast<size_t>(tm) * tb > kCntWords || static_cast<size_t>(tm) * tb * ksplit * BM * BN * 4 > kPartBytes) ksplit = 1;
+  XE_REQUIRE(ksplit == 1 || (static_cast<size_t>(tm) * tb <= kCntWords &&
+                             static_cast<size_t>(tm) * tb * ksplit * BM * BN * 4 <= kPartBytes),
+             "rows gemm: partial tiles beyond the workspace");
   const int blocks = (tm * tb * ksplit + kXcds - 1) / kXcds * kXcds;
-  hipLaunchKernelGGL((rows_tile_kernel<BM, BN>), dim3(blocks), dim3(256), 0, s, r, tm, tb, ksplit);
+  hipLaunchKernelGGL((rows_tile_kernel<BM, BN, WV>), dim3(blocks), dim3(64 * WV), 0, s, r, tm, tb, ksplit);
   XE_HIP(hipGetLastError());
 }
 
@@ -654,7 +642,7 @@ size_t rows_q8_ws_bytes() { return 2048 + kCntWords * 4 + kPartBytes; }
 
 size_t rows_q8_codes_bytes(int batch, int k) { return static_cast<size_t>(row_groups(batch)) * 16 * ((k + kStep - 1) / kStep * kStep); }
 
-void launch_rows_q8(const RowsQ8 &L, hipStream_t s) {
+int launch_rows_q8(const RowsQ8 &L, hipStream_t s) {
   RowsQ8 r = L;
   r.kp = (r.k + kStep - 1) / kStep * kStep;
   const int outs = r.a.act == XE_ACT_GEGLU ? r.m / 2 : r.m;
@@ -662,56 +650,32 @@ void launch_rows_q8(const RowsQ8 &L, hipStream_t s) {
                              reinterpret_cast<uintptr_t>(r.ws) | reinterpret_cast<uintptr_t>(r.bias)) & 15) == 0;
   const bool in16 = ((reinterpret_cast<uintptr_t>(r.a.x) | reinterpret_cast<uintptr_t>(r.a.add) | reinterpret_cast<uintptr_t>(r.a.sum) |
                       reinterpret_cast<uintptr_t>(r.a.post_w)) & 15) == 0;
-#ifndef XE_RQ_FW
-#define XE_RQ_FW 1, 1, 4, 8
-#endif
-#ifndef XE_RQ_FUSE
-#define XE_RQ_FUSE 1
-#endif
-  if (XE_RQ_FUSE && in16 && r.k <= 4096 && r.a.batch <= 16 && r.a.batch * r.kp <= kFusedBytes && !shares(r, outs)) {
-    if (r.k <= 1024) launch_gemm<XE_RQ_FW, 1>(r, s);
-    else if (r.k <= 2048) launch_gemm<XE_RQ_FW, 2>(r, s);
-    else launch_gemm<XE_RQ_FW, 4>(r, s);
-    return;
+  // One launch for one row: each workgroup makes the codes for itself, behind its
+  // first weight loads.  us in one launch / in two: 768 -> 768 4.9 / 6.7, 4096 ->
+  // 4096 9.4 / 11.2, 1152 -> 13824 8.4 / 11.8; two rows one after the other 6.2 /
+  // 6.6, 13.1 / 11.4, 10.9 / 11.9.
+  if (in16 && r.a.batch == 1 && r.k <= kFusedK && !shares(r, outs)) {
+    // 32 weight rows a workgroup instead of 16: 4.9 -> 5.1, 9.4 -> 10.8, 11.5 -> 8.4; 2048 -> 9000 9.8 -> 9.7
+    const bool wide = r.m > 32 * gdev::cu_count();
+    if (r.k <= 1024) wide ? launch_gemm<2, 1, 4, 4, 1>(r, s) : launch_gemm<1, 1, 4, 8, 1>(r, s);
+    else if (r.k <= 2048) wide ? launch_gemm<2, 1, 4, 4, 2>(r, s) : launch_gemm<1, 1, 4, 8, 2>(r, s);
+    else wide ? launch_gemm<2, 1, 4, 4, 4>(r, s) : launch_gemm<1, 1, 4, 8, 4>(r, s);
+    return 1;
   }
   if (in16) launch_quant<true>(r, s);
   else launch_quant<false>(r, s);
-#ifndef XE_RQ_V
-#define XE_RQ_V 0
-#endif
-  switch (XE_RQ_V) {
-    case 1: launch_gemm<1, 1, 4, 8>(r, s); return;
-    case 2: launch_gemm<1, 1, 8, 4>(r, s); return;
-    case 3: launch_gemm<1, 2, 4, 4>(r, s); return;
-    case 4: launch_gemm<1, 4, 4, 4>(r, s); return;
-    case 5: launch_gemm<1, 4, 8, 4>(r, s); return;
-    case 6: launch_gemm<2, 4, 4, 3>(r, s); return;
-    case 7: launch_gemm<4, 4, 4, 3>(r, s); return;
-    case 8: launch_gemm<4, 4, 4, 2>(r, s); return;
-    case 9: launch_gemm<8, 4, 4, 2>(r, s); return;
-    case 10: launch_gemm<4, 8, 4, 2>(r, s); return;
-    case 11: launch_gemm<2, 2, 4, 4>(r, s); return;
-    case 12: launch_gemm<8, 2, 4, 2>(r, s); return;
-    case 13: launch_gemm<2, 4, 8, 3>(r, s); return;
-    case 14: launch_gemm<4, 2, 4, 3>(r, s); return;
-    case 15: launch_gemm<2, 1, 4, 6>(r, s); return;
-    case 16: launch_gemm<2, 2, 8, 3>(r, s); return;
-    case 17: launch_gemm<4, 1, 4, 4>(r, s); return;
-    case 18: launch_gemm<1, 2, 8, 4>(r, s); return;
-    case 21: launch_tile<256, 128>(r, 1, s); return;
-    case 22: launch_tile<256, 128>(r, 2, s); return;
-    case 23: launch_tile<128, 128>(r, 1, s); return;
-    case 24: launch_tile<128, 128>(r, 2, s); return;
-    case 25: launch_tile<128, 128>(r, 4, s); return;
-    case 26: launch_tile<128, 64>(r, 1, s); return;
-    case 27: launch_tile<128, 64>(r, 2, s); return;
-    case 28: launch_tile<64, 64>(r, 1, s); return;
-    case 29: launch_tile<64, 64>(r, 2, s); return;
-    case 30: launch_tile<64, 64>(r, 4, s); return;
-    case 31: launch_tile<64, 128>(r, 1, s); return;
-    case 32: launch_tile<64, 128>(r, 2, s); return;
+  switch (rowsform::pick(r.m, r.k, r.a.batch, gdev::cu_count())) {
+    case 0: launch_gemm<1, 1, 4, 8>(r, s); break;
+    case 1: launch_gemm<1, 2, 4, 4>(r, s); break;
+    case 2: launch_gemm<2, 2, 4, 4>(r, s); break;
+    case 3: launch_tile<64, 64, 4>(r, 1, s); break;
+    case 4: launch_tile<64, 64, 4>(r, 2, s); break;
+    case 5: launch_tile<64, 64, 4>(r, 4, s); break;
+    case 6: launch_tile<128, 64, 8>(r, 1, s); break;
+    case 7: launch_tile<128, 128, 8>(r, 1, s); break;
+    default: launch_tile<256, 128, 8>(r, 1, s); break;
   }
-  launch_gemm<1, 4, 4, 4>(r, s);
+  return 2;
 }
 
 }  // namespace xe
