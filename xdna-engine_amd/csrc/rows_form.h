@@ -16,15 +16,15 @@ constexpr int kTiles = 1024;                     // tiles that have an arrival c
 // three have four waves that share K, 64 a step; the others take 128 a step and
 // split K, if at all, over workgroups.  Fitted to 288 shapes (m 768 to 14336, K
 // 768 to 14336, 8 to 512 rows), to 5 % a form.  The form of the least estimate is
-// 0.4 % slower than the fastest of all on average, 12 % at most.  Measured us,
-// with the quantisation, of the forms in the order of the table:
+// 0.4 % slower than the fastest of all on average, 12 % at most.  Measured us of
+// the forms in the order of the table (-: its partial tiles do not fit):
 //   m x K        rows
-//   4096 x 4096    16    12   12   14   17   16   17   20   24   34
-//   4096 x 4096    64    20   15   15   18   16   17   21   25   38
-//   4096 x 14336   64    46   33   30   40   31   28   48   63   94
-//   4096 x 14336  200   121   83   81   44   42   45   50   64   95
-//   14336 x 4096  200   134   88   76   37   40   36   32   29   41
-//   14336 x 4096  512   314  190  163   67   65   65   62   58   53
+//   4096 x 4096    16    6.2  6.7  8.9   12   10   11   14   19   28
+//   4096 x 4096    64     14  9.6  9.0   12   11   12   15   20   33
+//   4096 x 14336   64     37   23   20   30   21   18   38   53   84
+//   4096 x 14336  200    109   71   68   32   29   32   38   52   83
+//   14336 x 4096  200    128   81   70   31   34    -   26   23   35
+//   14336 x 4096  512    306  182  155   59    -    -   54   50   45
 struct Form {
   int bm, bn, ksplit, kstep;
   float fixed, step, round, out;

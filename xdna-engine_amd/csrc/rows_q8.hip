@@ -6,6 +6,8 @@
 // on the streams beside it (xe_w8a8_linear has one scale for all rows).
 // Statistics and rounding are in fp64, so that a code between two values does
 // not depend on the order of a sum: q and s are those of h itself.
+#include <type_traits>
+
 #include "attn_dev.h"
 #include "paged.h"
 #include "rows_form.h"
@@ -100,80 +102,96 @@ template <int NV, int T, bool VEC, typename Put>
 __device__ __forceinline__ float quant_row(const RowsQ8 &p, int b, bool writes, double (*red)[T / 64], Put &&put) {
   const int K = p.k, tid = threadIdx.x;
   const size_t at = static_cast<size_t>(b) * K;
-  f32x4 t[NV], su[NV], g[NV], be[NV];
+  // All loads of the row in flight at once where 4 waves a SIMD leave registers
+  // for them (128 each), otherwise the norms' where they are used.
+  constexpr bool kEarly = T < 1024;
+  f32x4 t[NV], su[NV], pw[NV], g[NV], be[NV];
+  auto load = [&](f32x4(&v)[NV], const float *src, auto vec) {
 #pragma unroll
-  for (int j = 0; j < NV; j++) {
-    const int i = 4 * (tid + T * j);
-    t[j] = su[j] = g[j] = be[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (i >= K) continue;
-    t[j] = load4<VEC>(p.a.x + at + i);
-    if (p.a.add) su[j] = load4<VEC>(p.a.add + at + i);
-    if (p.a.post_w) be[j] = load4<VEC>(p.a.post_w + i);
-  }
+    for (int j = 0; j < NV; j++) v[j] = load4<decltype(vec)::value>(src + min(4 * (tid + T * j), K - 4));
+  };
+  constexpr std::bool_constant<VEC> vec;
+  load(t, p.a.x + at, vec);
+  if (p.a.add) load(su, p.a.add + at, vec);
+  if (p.a.post_w) load(pw, p.a.post_w, vec);
+  if (kEarly && p.norm != XE_NORM_NONE) load(g, p.gamma, std::true_type{});
+  if (kEarly && p.norm == XE_NORM_LN) load(be, p.beta, std::true_type{});
   if (p.a.post_w) {
     double v = 0.0;
 #pragma unroll
     for (int j = 0; j < NV; j++)
 #pragma unroll
-      for (int c = 0; c < 4; c++) v += static_cast<double>(su[j][c]) * su[j][c];
+      for (int c = 0; c < 4; c++)
+        if (4 * (tid + T * j) < K) v = __builtin_fma(static_cast<double>(su[j][c]), static_cast<double>(su[j][c]), v);
     const double inv = 1.0 / sqrt(block_all<T>(v, red[0], Sum64{}) / K + static_cast<double>(p.a.post_eps));
 #pragma unroll
     for (int j = 0; j < NV; j++)
 #pragma unroll
-      for (int c = 0; c < 4; c++) su[j][c] = static_cast<float>(su[j][c] * inv * (1.0 + be[j][c]));
+      for (int c = 0; c < 4; c++) su[j][c] = static_cast<float>(su[j][c] * inv * (1.0 + pw[j][c]));
   }
+  if (p.a.add)
+#pragma unroll
+    for (int j = 0; j < NV; j++)
+#pragma unroll
+      for (int c = 0; c < 4; c++) t[j][c] += su[j][c];
 #pragma unroll
   for (int j = 0; j < NV; j++) {
     const int i = 4 * (tid + T * j);
-    if (i >= K) continue;
-    if (p.a.add)
-#pragma unroll
-      for (int c = 0; c < 4; c++) t[j][c] += su[j][c];
-    if (p.a.sum && writes) {
+    if (p.a.sum && writes && i < K) {
       if constexpr (VEC) *reinterpret_cast<f32x4 *>(p.a.sum + at + i) = t[j];
       else
 #pragma unroll
         for (int c = 0; c < 4; c++) p.a.sum[at + i + c] = t[j][c];
     }
-    if (p.norm != XE_NORM_NONE) g[j] = *reinterpret_cast<const f32x4 *>(p.gamma + i);
-    if (p.norm == XE_NORM_LN) be[j] = *reinterpret_cast<const f32x4 *>(p.beta + i);
+    if (i >= K) t[j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  double mean = 0.0, inv = 1.0;
-  const double one = p.norm == XE_NORM_RMS1P ? 1.0 : 0.0;
+  double h[NV][4];
+#pragma unroll
+  for (int j = 0; j < NV; j++)
+#pragma unroll
+    for (int c = 0; c < 4; c++) h[j][c] = t[j][c];
   if (p.norm != XE_NORM_NONE) {
+    if (!kEarly) load(g, p.gamma, std::true_type{});
     double v = 0.0;
     if (p.norm == XE_NORM_LN) {
 #pragma unroll
       for (int j = 0; j < NV; j++)
 #pragma unroll
-        for (int c = 0; c < 4; c++) v += t[j][c];
-      mean = block_all<T>(v, red[1], Sum64{}) / K;
+        for (int c = 0; c < 4; c++) v += h[j][c];
+      const double mean = block_all<T>(v, red[1], Sum64{}) / K;
       v = 0.0;
+#pragma unroll
+      for (int j = 0; j < NV; j++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) h[j][c] = 4 * (tid + T * j) < K ? h[j][c] - mean : 0.0;
     }
 #pragma unroll
     for (int j = 0; j < NV; j++)
 #pragma unroll
-      for (int c = 0; c < 4; c++)
-        if (4 * (tid + T * j) < K) v += (t[j][c] - mean) * (t[j][c] - mean);
-    inv = 1.0 / sqrt(block_all<T>(v, red[2], Sum64{}) / K + static_cast<double>(p.eps));
+      for (int c = 0; c < 4; c++) v = __builtin_fma(h[j][c], h[j][c], v);
+    const double inv = 1.0 / sqrt(block_all<T>(v, red[2], Sum64{}) / K + static_cast<double>(p.eps));
+    const double one = p.norm == XE_NORM_RMS1P ? 1.0 : 0.0;
+#pragma unroll
+    for (int j = 0; j < NV; j++)
+#pragma unroll
+      for (int c = 0; c < 4; c++) h[j][c] = h[j][c] * inv * (one + g[j][c]);
+    if (p.norm == XE_NORM_LN) {
+      if (!kEarly) load(be, p.beta, std::true_type{});
+#pragma unroll
+      for (int j = 0; j < NV; j++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) h[j][c] = 4 * (tid + T * j) < K ? h[j][c] + be[j][c] : 0.0;
+    }
   }
-  auto h = [&](int j, int c) {
-    if (p.norm == XE_NORM_NONE) return static_cast<double>(t[j][c]);
-    const double v = (t[j][c] - mean) * inv * (one + g[j][c]);
-    return p.norm == XE_NORM_LN ? v + be[j][c] : v;
-  };
-  double a = 0.0;
-  bool bad = false;
+  double a = 0.0, bad = 0.0;  // bad: NaN once a value is NaN or infinite
 #pragma unroll
   for (int j = 0; j < NV; j++)
 #pragma unroll
     for (int c = 0; c < 4; c++) {
-      if (4 * (tid + T * j) >= K) continue;
-      const double v = fabs(h(j, c));
-      bad |= !(v <= 1.7976931348623157e308);
-      a = fmax(a, v);
+      a = fmax(a, fabs(h[j][c]));
+      bad = __builtin_fma(h[j][c], 0.0, bad);
     }
-  const double amax = block_all<T>(bad ? INFINITY : a, red[3], Max64{});
+  const double amax = block_all<T>(bad == 0.0 ? a : INFINITY, red[3], Max64{});
   float s = static_cast<float>(amax / 127.0);
   if (!(s > 0.f)) s = 1.f;
   const bool number = s < INFINITY;  // else NaN or infinity in the row: its scale, and its outputs, become NaN
@@ -184,17 +202,22 @@ __device__ __forceinline__ float quant_row(const RowsQ8 &p, int b, bool writes, 
     if (i >= p.kp) continue;
     uint32_t q = 0;
 #pragma unroll
-    for (int c = 0; c < 4; c++) {
-      const int code = static_cast<int>(fmin(fmax(round(h(j, c) * r), -127.0), 127.0));
-      q |= (static_cast<uint32_t>(code) & 0xffu) << (8 * c);
+    for (int c = 0; c < 4; c++) {  // half a unit away from zero, then cut; a scale below fp32's normal range may leave more than 127
+      const int code = static_cast<int>(__builtin_fma(h[j][c], r, copysign(0.5, h[j][c])));
+      q |= (static_cast<uint32_t>(min(max(code, -127), 127)) & 0xffu) << (8 * c);
     }
     put(i, number && i < K ? q : 0u);
   }
   return number ? s : NAN;
 }
 
-// One workgroup a row.  Bound by the rows' bytes where they are many, by the
-// chain of a load and two or three block reductions where they are few.
+// One workgroup a row, as few threads as hold it in 16 elements each.  Bound by
+// the chain of a load and two or three block reductions where rows are few (64 of
+// 4096: 3.5 us), by fp64 instructions where they are many (512 of 4096 8.6, 200 of
+// 14336 7.3; the rows' bytes 2.2 and 3).  Rounding by a multiply-add and a
+// conversion, loads all ahead and h kept took these from 4.9, 11.0 and 9.6.  Half
+// the threads with twice the elements: 200 of 14336 1.4 us more; twice the
+// threads: 300 of 8192 0.7 more.  K beyond 16384 spills 90 registers.
 template <int NV, int T, bool VEC>
 __global__ __launch_bounds__(T) void rows_quant_kernel(RowsQ8 p) {
   __shared__ double red[4][T / 64];
@@ -651,11 +674,11 @@ int launch_rows_q8(const RowsQ8 &L, hipStream_t s) {
   const bool in16 = ((reinterpret_cast<uintptr_t>(r.a.x) | reinterpret_cast<uintptr_t>(r.a.add) | reinterpret_cast<uintptr_t>(r.a.sum) |
                       reinterpret_cast<uintptr_t>(r.a.post_w)) & 15) == 0;
   // One launch for one row: each workgroup makes the codes for itself, behind its
-  // first weight loads.  us in one launch / in two: 768 -> 768 4.9 / 6.7, 4096 ->
-  // 4096 9.4 / 11.2, 1152 -> 13824 8.4 / 11.8; two rows one after the other 6.2 /
-  // 6.6, 13.1 / 11.4, 10.9 / 11.9.
+  // first weight loads.  us in one launch / in two: 768 -> 768 4.4 / 6.2, 4096 ->
+  // 4096 7.4 / 9.0, 1152 -> 13824 7.5 / 10.6.  Two rows one after the other took
+  // longer than two launches where K is 4096.
   if (in16 && r.a.batch == 1 && r.k <= kFusedK && !shares(r, outs)) {
-    // 32 weight rows a workgroup instead of 16: 4.9 -> 5.1, 9.4 -> 10.8, 11.5 -> 8.4; 2048 -> 9000 9.8 -> 9.7
+    // 32 weight rows a workgroup / 16: those 4.8 / 4.4, 8.9 / 7.4, 7.5 / 8.2; 2048 -> 9000 8.6 / 8.4
     const bool wide = r.m > 32 * gdev::cu_count();
     if (r.k <= 1024) wide ? launch_gemm<2, 1, 4, 4, 1>(r, s) : launch_gemm<1, 1, 4, 8, 1>(r, s);
     else if (r.k <= 2048) wide ? launch_gemm<2, 1, 4, 4, 2>(r, s) : launch_gemm<1, 1, 4, 8, 2>(r, s);
