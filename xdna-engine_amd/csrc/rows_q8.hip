@@ -312,7 +312,10 @@ struct Epi4 {
 // waves each over their own part of K (v_mfma_i32_16x16x64_i8: a lane holds 16
 // consecutive k of weight row lane % 16 and of activation row lane % 16), U
 // steps of 64 in flight.  NV > 0: the workgroup makes the codes itself (K <= 1024
-// NV, one row), into LDS, while its first weights load.
+// NV, one row), into LDS, while its first weights load.  Bound by the weights'
+// way to the CUs: 64 x 4096 -> 4096 7.3 us for 17 MB of weights (3.5 at a large
+// copy's 4.86 TB/s) that two tiles of rows each read; one row 1152 -> 13824 6.4 for
+// 16 MB.  Sums meet in LDS: one round, no other workgroup to wait for.
 template <int WR, int NJ, int KS, int U, int NV>
 __global__ __launch_bounds__(64 * KS) void rows_gemm_kernel(RowsQ8 p, int ntile_m, int ntile_b) {
   constexpr int NB = WR * NJ;                     // 16 x 16 blocks
@@ -440,6 +443,13 @@ __device__ __forceinline__ void rows_out(const RowsQ8 &p, const int *sums, int s
 // x BN / 2; K in steps of 128 bytes through two LDS buffers, the loads of two
 // more steps in registers.  Rows lie 128 bytes apart in LDS, their 16-byte
 // chunks permuted by the row, so that 16 rows read together cover all banks.
+// Parts of K (ksplit) leave their sums in `part`; the last workgroup of a tile to
+// arrive adds them, integers, so that their order changes nothing.  Bound by the
+// matrix instructions: 512 x 4096 -> 14336 in 256 x 128 tiles 41.5 us, 1450 TOP/s on
+// 224 of 256 CUs (a large int8 product reaches 1781 on all).  Smaller tiles by
+// what the CUs load: 200 x 14336 -> 4096 in 64 x 64 tiles and two parts of K 29.8
+// us for 470 MB of operands out of L2, 16 TB/s (runs of 128 bytes reach 17 to 20).
+// Eight waves instead of four, 128 x 64 tiles, 512 x 4096 -> 4096: 28.6 -> 27.3.
 template <int BM, int BN, int WV>
 __global__ __launch_bounds__(64 * WV, 2) void rows_tile_kernel(RowsQ8 p, int ntile_m, int ntile_b, int ksplit) {
   constexpr int T = 64 * WV, MW = BM / (WV / 2), NW = BN / 2;  // a wave's rows of weights, of activations
