@@ -180,12 +180,12 @@ int main() {
           assert(i >= 0 && i < kForms && fits(i, m, batch));
         }
   for (int i = 0; i < kForms; i++)
-    if (kForm[i].ksplit > 1 && i >= kInWaves) {
+    if (kForm[i].ksplit > 1) {
       assert(fits(i, kForm[i].bm, kForm[i].bn) && !fits(i, 134217727, 512));
       assert(!fits(i, kForm[i].bm * (kTiles + 1), 1));
     }
   const int tests[][3] = {{200, 192, 3},     {200, 192, 512},   {301, 720, 509},  {702, 160, 511},   {702, 4112, 397},
-                          {702, 8208, 197}, {2102, 304, 509}, {4102, 1040, 510}, {8200, 8208, 449}};
+                          {702, 8208, 197}, {2102, 304, 509}, {4102, 1040, 510}, {14402, 4112, 400}, {97, 8208, 5}, {97, 8208, 200}};
   for (auto &t : tests) seen[pick(t[0], t[1], t[2], 256)]++;
   for (int n : seen) assert(n == 1);
 }

@@ -69,7 +69,8 @@ def test_shapes(gpu, xe, m, k, batch):
 
 
 @pytest.mark.parametrize("m,k,batch", [(301, 720, 509), (702, 160, 511), (702, 4112, 397), (702, 8208, 197), (2102, 304, 509),
-                                       (4102, 1040, 510), (8200, 8208, 449)])
+                                       (4102, 1040, 510), (8200, 8208, 449), (14402, 4112, 400), (97, 8208, 5),
+                                       (97, 8208, 200)])
 @pytest.mark.parametrize("act", [1, 4])
 def test_larger_shapes(gpu, xe, m, k, batch, act):
     """Every form of the product, with tiles that end outside in both directions."""

@@ -20,6 +20,7 @@ constexpr unsigned kNoRec = 0x7ffffff0u;  // past every buffer: loads return zer
 constexpr int kXcds = 8;
 constexpr size_t kPartBytes = rowsform::kPartBytes;  // partial tiles of K splits
 constexpr size_t kCntWords = rowsform::kTiles;       // and their arrival counters
+constexpr int kMaxSplit = 4;        // parts of K
 constexpr int kStep = 128;          // bytes of K a step
 constexpr int kFusedK = 4096;       // K up to which a workgroup makes one row's codes itself
 
@@ -315,23 +316,27 @@ struct Epi4 {
 // NV, one row), into LDS, while its first weights load.  Bound by the weights'
 // way to the CUs: 64 x 4096 -> 4096 7.3 us for 17 MB of weights (3.5 at a large
 // copy's 4.86 TB/s) that two tiles of rows each read; one row 1152 -> 13824 6.4 for
-// 16 MB.  Sums meet in LDS: one round, no other workgroup to wait for.
+// 16 MB.  The waves' sums meet in LDS.  A CU draws such rows of 64 bytes at 37 B/ns,
+// so that few tiles of a long K are bound by that: parts of K (ksplit) go to
+// other CUs then and leave their sums in `part`; the last workgroup of a tile to
+// arrive adds them, integers, so that their order changes nothing.
 template <int WR, int NJ, int KS, int U, int NV>
-__global__ __launch_bounds__(64 * KS) void rows_gemm_kernel(RowsQ8 p, int ntile_m, int ntile_b) {
+__global__ __launch_bounds__(64 * KS) void rows_gemm_kernel(RowsQ8 p, int ntile_m, int ntile_b, int ksplit) {
   constexpr int NB = WR * NJ;                     // 16 x 16 blocks
   constexpr bool kFused = NV > 0;
   static_assert(!kFused || (KS == 4 && NJ == 1), "one row made here by 256 threads");
   __shared__ __attribute__((aligned(16))) int part[KS][NB][256];
   __shared__ __attribute__((aligned(16))) int8_t codes[kFused ? kFusedK : 16];
   __shared__ double red[kFused ? 4 : 1][4];
+  __shared__ int flag;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 15, lg = lane >> 4;
-  // The tiles of an XCD lie in a row, those of the same weight rows next to
-  // each other: its L2 reads the weights once.
-  const int all = ntile_m * ntile_b, each = (all + kXcds - 1) / kXcds;
-  const int tile = static_cast<int>(blockIdx.x % kXcds) * each + static_cast<int>(blockIdx.x / kXcds);
-  if (static_cast<int>(blockIdx.x / kXcds) >= each || tile >= all) return;
-  const int tm = tile / ntile_b, tb = tile - tm * ntile_b;
+  // The tiles of an XCD lie in a row, those of the same weights next to each
+  // other: its L2 reads the weights once.
+  const int all = ntile_m * ntile_b * ksplit, each = (all + kXcds - 1) / kXcds;
+  const int at = static_cast<int>(blockIdx.x % kXcds) * each + static_cast<int>(blockIdx.x / kXcds);
+  if (static_cast<int>(blockIdx.x / kXcds) >= each || at >= all) return;
+  const int tb = at % ntile_b, rest = at / ntile_b, kz = rest % ksplit, tm = rest / ksplit;
   const int r0 = tm * 16 * WR, b0 = tb * 16 * NJ;
   const int kp = p.kp;
   const __amdgpu_buffer_rsrc_t rw = bounded_rsrc(p.w, static_cast<unsigned>(p.m) * p.k);
@@ -342,8 +347,8 @@ __global__ __launch_bounds__(64 * KS) void rows_gemm_kernel(RowsQ8 p, int ntile_
   for (int r = 0; r < WR; r++) wo[r] = r0 + 16 * r + ln < p.m ? static_cast<unsigned>(r0 + 16 * r + ln) * p.k + 16 * lg : kNoRec;
 #pragma unroll
   for (int j = 0; j < NJ; j++) xo[j] = tb * NJ + j < groups ? static_cast<unsigned>(tb * NJ + j) * 1024 + 16 * lane : kNoRec;
-  const int steps = (p.k + 63) / 64, q = steps / KS, rem = steps % KS;
-  const int s0 = q * wave + min(wave, rem), s1 = s0 + q + (wave < rem ? 1 : 0);
+  const int steps = (p.k + 63) / 64, slot = kz * KS + wave, q = steps / (KS * ksplit), rem = steps % (KS * ksplit);
+  const int s0 = q * slot + min(slot, rem), s1 = s0 + q + (slot < rem ? 1 : 0);
   i32x4 w[U][WR], x[U][NJ];
   auto issue = [&](int u, int s) {  // past the last step: zeros
     const bool ok = s < s1;
@@ -366,7 +371,7 @@ __global__ __launch_bounds__(64 * KS) void rows_gemm_kernel(RowsQ8 p, int ntile_
   Epi4 epi;
   if (wave < NB) epi.load(p, ob, orow, !kFused);
   if constexpr (kFused) {
-    epi.s = quant_row<NV, 256, true>(p, 0, tile == 0, red, [&](int i, uint32_t c) { *reinterpret_cast<uint32_t *>(codes + i) = c; });
+    epi.s = quant_row<NV, 256, true>(p, 0, at == 0, red, [&](int i, uint32_t c) { *reinterpret_cast<uint32_t *>(codes + i) = c; });
     __syncthreads();
   }
   for (int s = s0; s < s1; s += U) {
@@ -384,17 +389,43 @@ __global__ __launch_bounds__(64 * KS) void rows_gemm_kernel(RowsQ8 p, int ntile_
 #pragma unroll
   for (int i = 0; i < NB; i++) *reinterpret_cast<i32x4 *>(&part[wave][i][4 * lane]) = acc[i];
   __syncthreads();
-  for (int i = wave; i < NB; i += KS) {
+  auto waves_sum = [&](int i) {
     i32x4 sum = *reinterpret_cast<const i32x4 *>(&part[0][i][4 * lane]);
 #pragma unroll
     for (int k = 1; k < KS; k++) {
       const i32x4 v = *reinterpret_cast<const i32x4 *>(&part[k][i][4 * lane]);
 #pragma unroll
-      for (int z = 0; z < 4; z++) sum[z] += v[z];
+      for (int c = 0; c < 4; c++) sum[c] += v[c];
     }
+    return sum;
+  };
+  auto finish = [&](int i, const i32x4 &sum) {
     const int b = b0 + 16 * (i % NJ) + ln, r = r0 + 16 * (i / NJ) + 4 * lg;
     if (i != wave) epi.load(p, b, r, !kFused);
     if (b < p.a.batch && r < p.m) epi.finish(p, b, r, sum);
+  };
+  if (kFused || ksplit == 1) {
+    for (int i = wave; i < NB; i += KS) finish(i, waves_sum(i));
+    return;
+  }
+  const size_t tile = static_cast<size_t>(tm) * ntile_b + tb;
+  const __amdgpu_buffer_rsrc_t rp = gdev::coherent_rsrc(reinterpret_cast<const i32x4 *>(p.part) + tile * ksplit * NB * 64);
+  for (int i = wave; i < NB; i += KS)
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, waves_sum(i)), rp, ((kz * NB + i) * 64 + lane) * 16, 0,
+                                           gdev::kCoherentSc1);
+  if (!adev::last_to_arrive(p.cnt + tile, ksplit, &flag)) return;
+  if (threadIdx.x == 0) __hip_atomic_store(p.cnt + tile, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  for (int i = wave; i < NB; i += KS) {
+    i32x4 v[kMaxSplit], sum = {0, 0, 0, 0};
+#pragma unroll
+    for (int o = 0; o < kMaxSplit; o++)  // past the last one: that one again, not added
+      v[o] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rp, ((min(o, ksplit - 1) * NB + i) * 64 + lane) * 16, 0,
+                                                                             gdev::kCoherentSc1));
+#pragma unroll
+    for (int o = 0; o < kMaxSplit; o++)
+#pragma unroll
+      for (int c = 0; c < 4; c++) sum[c] += o < ksplit ? v[o][c] : 0;
+    finish(i, sum);
   }
 }
 
@@ -443,8 +474,7 @@ __device__ __forceinline__ void rows_out(const RowsQ8 &p, const int *sums, int s
 // x BN / 2; K in steps of 128 bytes through two LDS buffers, the loads of two
 // more steps in registers.  Rows lie 128 bytes apart in LDS, their 16-byte
 // chunks permuted by the row, so that 16 rows read together cover all banks.
-// Parts of K (ksplit) leave their sums in `part`; the last workgroup of a tile to
-// arrive adds them, integers, so that their order changes nothing.  Bound by the
+// Parts of K as above.  Bound by the
 // matrix instructions: 512 x 4096 -> 14336 in 256 x 128 tiles 41.5 us, 1450 TOP/s on
 // 224 of 256 CUs (a large int8 product reaches 1781 on all).  Smaller tiles by
 // what the CUs load: 200 x 14336 -> 4096 in 64 x 64 tiles and two parts of K 29.8
@@ -626,20 +656,27 @@ __global__ __launch_bounds__(64 * WV, 2) void rows_tile_kernel(RowsQ8 p, int nti
   }
 }
 
+// Parts of K leave tiles of bm x bn sums in the workspace.
+void check_split(int tm, int tb, int ksplit, int bm, int bn) {
+  const int64_t tiles = static_cast<int64_t>(tm) * tb;
+  XE_REQUIRE(ksplit == 1 || (ksplit <= kMaxSplit && tiles <= static_cast<int64_t>(kCntWords) &&
+                             tiles * ksplit * bm * bn * 4 <= static_cast<int64_t>(kPartBytes)),
+             "rows gemm: partial tiles beyond the workspace");
+}
+
 template <int WR, int NJ, int KS, int U, int NV = 0>
-void launch_gemm(const RowsQ8 &r, hipStream_t s) {
+void launch_gemm(const RowsQ8 &r, int ksplit, hipStream_t s) {
   const int tm = (r.m + 16 * WR - 1) / (16 * WR), tb = (r.a.batch + 16 * NJ - 1) / (16 * NJ);
-  const int blocks = (tm * tb + kXcds - 1) / kXcds * kXcds;
-  hipLaunchKernelGGL((rows_gemm_kernel<WR, NJ, KS, U, NV>), dim3(blocks), dim3(64 * KS), 0, s, r, tm, tb);
+  check_split(tm, tb, ksplit, 16 * WR, 16 * NJ);
+  const int blocks = (tm * tb * ksplit + kXcds - 1) / kXcds * kXcds;
+  hipLaunchKernelGGL((rows_gemm_kernel<WR, NJ, KS, U, NV>), dim3(blocks), dim3(64 * KS), 0, s, r, tm, tb, ksplit);
   XE_HIP(hipGetLastError());
 }
 
 template <int BM, int BN, int WV>
 void launch_tile(const RowsQ8 &r, int ksplit, hipStream_t s) {
   const int tm = (r.m + BM - 1) / BM, tb = (r.a.batch + BN - 1) / BN;
-  XE_REQUIRE(ksplit == 1 || (static_cast<size_t>(tm) * tb <= kCntWords &&
-                             static_cast<size_t>(tm) * tb * ksplit * BM * BN * 4 <= kPartBytes),
-             "rows gemm: partial tiles beyond the workspace");
+  check_split(tm, tb, ksplit, BM, BN);
   const int blocks = (tm * tb * ksplit + kXcds - 1) / kXcds * kXcds;
   hipLaunchKernelGGL((rows_tile_kernel<BM, BN, WV>), dim3(blocks), dim3(64 * WV), 0, s, r, tm, tb, ksplit);
   XE_HIP(hipGetLastError());
@@ -690,23 +727,25 @@ int launch_rows_q8(const RowsQ8 &L, hipStream_t s) {
   if (in16 && r.a.batch == 1 && r.k <= kFusedK && !shares(r, outs)) {
     // 32 weight rows a workgroup / 16: those 4.8 / 4.4, 8.9 / 7.4, 7.5 / 8.2; 2048 -> 9000 8.6 / 8.4
     const bool wide = r.m > 32 * gdev::cu_count();
-    if (r.k <= 1024) wide ? launch_gemm<2, 1, 4, 4, 1>(r, s) : launch_gemm<1, 1, 4, 8, 1>(r, s);
-    else if (r.k <= 2048) wide ? launch_gemm<2, 1, 4, 4, 2>(r, s) : launch_gemm<1, 1, 4, 8, 2>(r, s);
-    else wide ? launch_gemm<2, 1, 4, 4, 4>(r, s) : launch_gemm<1, 1, 4, 8, 4>(r, s);
+    if (r.k <= 1024) wide ? launch_gemm<2, 1, 4, 4, 1>(r, 1, s) : launch_gemm<1, 1, 4, 8, 1>(r, 1, s);
+    else if (r.k <= 2048) wide ? launch_gemm<2, 1, 4, 4, 2>(r, 1, s) : launch_gemm<1, 1, 4, 8, 2>(r, 1, s);
+    else wide ? launch_gemm<2, 1, 4, 4, 4>(r, 1, s) : launch_gemm<1, 1, 4, 8, 4>(r, 1, s);
     return 1;
   }
   if (in16) launch_quant<true>(r, s);
   else launch_quant<false>(r, s);
   switch (rowsform::pick(r.m, r.k, r.a.batch, gdev::cu_count())) {
-    case 0: launch_gemm<1, 1, 4, 8>(r, s); break;
-    case 1: launch_gemm<1, 2, 4, 4>(r, s); break;
-    case 2: launch_gemm<2, 2, 4, 4>(r, s); break;
+    case 0: launch_gemm<1, 1, 4, 8>(r, 1, s); break;
+    case 1: launch_gemm<1, 2, 4, 4>(r, 1, s); break;
+    case 2: launch_gemm<2, 2, 4, 4>(r, 1, s); break;
     case 3: launch_tile<64, 64, 4>(r, 1, s); break;
     case 4: launch_tile<64, 64, 4>(r, 2, s); break;
     case 5: launch_tile<64, 64, 4>(r, 4, s); break;
     case 6: launch_tile<128, 64, 8>(r, 1, s); break;
     case 7: launch_tile<128, 128, 8>(r, 1, s); break;
-    default: launch_tile<256, 128, 8>(r, 1, s); break;
+    case 8: launch_tile<256, 128, 8>(r, 1, s); break;
+    case 9: launch_gemm<1, 1, 4, 8>(r, 4, s); break;
+    default: launch_gemm<1, 2, 4, 4>(r, 4, s); break;
   }
   return 2;
 }
