@@ -382,7 +382,7 @@ typedef struct xe_w8a8_rows {
  * step in fp32 (infinite where it leaves fp32's range).  Unlike xe_w8a8_linear, whose
  * one scale spans all rows (ctx2.rs:1352-1377), a row's result does not depend
  * on the rows beside it.  A row with a NaN or an infinity in h gives NaN.
- * K up to 32768. */
+ * K up to 32768, weights below 2 GB, views 16-byte aligned. */
 int xe_w8a8_rows_dev(xe_ctx *ctx, const xe_weight *w, const xe_w8a8_rows *rows);
 
 /* Wait for the ctx stream; returns 0 or -1. */

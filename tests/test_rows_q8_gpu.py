@@ -180,9 +180,44 @@ def test_refusals_over_weights(gpu, xe):
     odd = ctx.register_weight_q8(np.ones((3, 16), np.int8), np.ones(3, np.float32))
     wide = ctx.register_weight_q8(np.ones((1, 32784), np.int8), np.ones(1, np.float32))
     half = ctx.register_weight(np.ones((4, 16), np.float32), wdtype=xe.XE_BF16)
-    for w, act in ((odd, xe.XE_ACT_GEGLU), (wide, 0), (half, 0)):
+    tilted = ctx.register_weight_view(xe.XE_I8, 4, 16, b.ptr + 8, scale_ptr=b.ptr)
+    for w, act in ((odd, xe.XE_ACT_GEGLU), (wide, 0), (half, 0), (tilted, 0)):
         with pytest.raises(xe.XdnaError):
             ctx.w8a8_rows_dev(w, xe.W8a8Rows(1, b.ptr, b.ptr, act=act))
-    for w in (odd, wide, half):
+    for w in (odd, wide, half, tilted):
         w.free()
     b.free()
+
+
+@pytest.mark.parametrize("batch", [1, 2, 20, 90, 300])
+@pytest.mark.parametrize("off", [1, 2, 4])
+def test_addresses(gpu, xe, batch, off):
+    """Rows, results and a weight view's scales and bias at addresses off by 4, 8
+    and 16 bytes from a multiple of 32; what lies around the results stays."""
+    dev, ctx = gpu
+    rng = np.random.default_rng(batch + off)
+    m, k = 264, 1040
+    q8 = rng.integers(-127, 128, (m, k)).astype(np.int8)
+    ws, bias = rng.uniform(0.001, 0.02, m).astype(np.float32), rng.standard_normal(m).astype(np.float32)
+    x, add = (rng.standard_normal((batch, k)).astype(np.float32) for _ in range(2))
+    pw, res = (0.2 * rng.standard_normal(k)).astype(np.float32), rng.standard_normal((batch, m)).astype(np.float32)
+    gamma = (1 + 0.2 * rng.standard_normal(k)).astype(np.float32)
+
+    def shifted(a):
+        return put(xe, dev, np.concatenate([np.full(off, 9.0, np.float32), a.reshape(-1), np.full(8, 9.0, np.float32)]))
+    bufs = [shifted(a) for a in (ws, bias, x, add, pw, res, np.zeros((batch, k), np.float32), np.zeros((batch, m), np.float32))]
+    bw = put(xe, dev, q8)
+    pws, pbias, px, padd, ppost, pres, psum, py = (b.ptr + 4 * off for b in bufs)
+    w = ctx.register_weight_view(xe.XE_I8, m, k, bw.ptr, scale_ptr=pws, bias_ptr=pbias)
+    ctx.set_norm(w, xe.Norm(2, gamma, np.zeros(k, np.float32), 1e-6))
+    ctx.w8a8_rows_dev(w, xe.W8a8Rows(batch, px, py, act=xe.XE_ACT_RELU, add=padd, post_w=ppost, sum=psum, res=pres))
+    ctx.synchronize()
+    want, t, bound = rows64(q8, ws, bias, 2, gamma, None, 1e-6, x, add, pw, 1, res)
+    for b, n, check in ((bufs[7], batch * m, lambda g: within(g.reshape(batch, m), want, bound, "rows")),
+                        (bufs[6], batch * k, lambda g: within(g.reshape(batch, k), t.astype(np.float64), 2 ** -23 * np.abs(t) + 1e-30, "sum"))):
+        got = b.read(np.float32, off + n + 8)
+        assert np.all(got[:off] == 9.0) and np.all(got[off + n:] == 9.0)
+        check(got[off:off + n])
+    w.free()
+    for b in (*bufs, bw):
+        b.free()

@@ -127,7 +127,7 @@ template <int HD>
 void launch_hd(const AppendParams &p, bool vec, hipStream_t s) {
   constexpr int GROUPS = kT / (HD / 8);
   const long long blocks = (static_cast<long long>(p.r.n_rows) * p.heads + GROUPS - 1) / GROUPS;
-  XE_REQUIRE(blocks < (1LL << 31), "paged append: too many rows");
+  XE_REQUIRE(blocks * kT < (1LL << 32), "paged append: too many rows for one launch");
   hipLaunchKernelGGL((vec ? append_kernel<HD, true> : append_kernel<HD, false>), dim3(static_cast<unsigned>(blocks)),
                      dim3(kT), 0, s, p);
   XE_HIP(hipGetLastError());

@@ -657,8 +657,9 @@ __global__ __launch_bounds__(64 * WV, 2) void rows_tile_kernel(RowsQ8 p, int nti
 }
 
 // Parts of K leave tiles of bm x bn sums in the workspace.
-void check_split(int tm, int tb, int ksplit, int bm, int bn) {
+void check_tiles(int tm, int tb, int ksplit, int bm, int bn) {
   const int64_t tiles = static_cast<int64_t>(tm) * tb;
+  XE_REQUIRE(tiles * ksplit <= (1 << 22), "rows gemm: too many tiles for one launch");
   XE_REQUIRE(ksplit == 1 || (ksplit <= kMaxSplit && tiles <= static_cast<int64_t>(kCntWords) &&
                              tiles * ksplit * bm * bn * 4 <= static_cast<int64_t>(kPartBytes)),
              "rows gemm: partial tiles beyond the workspace");
@@ -667,7 +668,7 @@ void check_split(int tm, int tb, int ksplit, int bm, int bn) {
 template <int WR, int NJ, int KS, int U, int NV = 0>
 void launch_gemm(const RowsQ8 &r, int ksplit, hipStream_t s) {
   const int tm = (r.m + 16 * WR - 1) / (16 * WR), tb = (r.a.batch + 16 * NJ - 1) / (16 * NJ);
-  check_split(tm, tb, ksplit, 16 * WR, 16 * NJ);
+  check_tiles(tm, tb, ksplit, 16 * WR, 16 * NJ);
   const int blocks = (tm * tb * ksplit + kXcds - 1) / kXcds * kXcds;
   hipLaunchKernelGGL((rows_gemm_kernel<WR, NJ, KS, U, NV>), dim3(blocks), dim3(64 * KS), 0, s, r, tm, tb, ksplit);
   XE_HIP(hipGetLastError());
@@ -676,7 +677,7 @@ void launch_gemm(const RowsQ8 &r, int ksplit, hipStream_t s) {
 template <int BM, int BN, int WV>
 void launch_tile(const RowsQ8 &r, int ksplit, hipStream_t s) {
   const int tm = (r.m + BM - 1) / BM, tb = (r.a.batch + BN - 1) / BN;
-  check_split(tm, tb, ksplit, BM, BN);
+  check_tiles(tm, tb, ksplit, BM, BN);
   const int blocks = (tm * tb * ksplit + kXcds - 1) / kXcds * kXcds;
   hipLaunchKernelGGL((rows_tile_kernel<BM, BN, WV>), dim3(blocks), dim3(64 * WV), 0, s, r, tm, tb, ksplit);
   XE_HIP(hipGetLastError());
