@@ -268,6 +268,43 @@ def test_attn_many_streams(gpu, xe, batch):
     attn_case(xe, gpu, batch, 2, 1, 64, 16, lens, 6)
 
 
+def test_attn_most_streams(gpu, xe):
+    rng = np.random.default_rng(4096)
+    attn_case(xe, gpu, 24, 2, 1, 64, 16, rng.choice([0, 1, 16, 17, 32], 4096), 2)
+
+
+@pytest.mark.parametrize("hq,hkv,batch", [(1024, 1, 2), (1024, 1, 70), (1024, 1024, 3), (48, 16, 2), (48, 16, 70)])
+def test_attn_many_heads(gpu, xe, hq, hkv, batch):
+    attn_case(xe, gpu, hq + hkv, hq, hkv, 64, 16, [18, 3] * (batch // 2) + [0] * (batch % 2), 2)
+
+
+@pytest.mark.parametrize("hq,hkv,hd", [(2, 1, 64), (20, 1, 128)])
+def test_attn_one_long_stream_among_short_ones(gpu, xe, hq, hkv, hd):
+    """Its partials meet on three levels; the others read its first page."""
+    dev, ctx = gpu
+    print("[case] one stream of 60001 keys among 65, %d/%d x %d" % (hq, hkv, hd), flush=True)
+    rng = np.random.default_rng(25)
+    page, n, batch = 256, 60001, 65
+    c = Cache(xe, dev, rng, 1, -(-n // page), page, hkv, hd)
+    table = np.full((batch, c.table.shape[1]), -1, np.int32)
+    table[30] = c.table[0]
+    table[:, 0] = c.table[0, 0]
+    c.table, c.dims = table, (batch,) + c.dims[1:]
+    lens = np.arange(batch, dtype=np.int32) % 17
+    lens[30] = n
+    q = rng.standard_normal((batch, hq, hd)).astype(np.float32)
+    kv = c.upload()
+    bufs = [put(xe, dev, a) for a in (q, lens, np.full(q.shape, 3.25, np.float32))]
+    want, bound = attn64(c, q, lens, hq, hd ** -0.5)
+    for _ in range(3):
+        ctx.paged_attn_dev(kv, bufs[0], bufs[1], hq, hd ** -0.5, bufs[2])
+        ctx.synchronize()
+        within(bufs[2].read(np.float32, q.size).reshape(q.shape), want, bound, "attention")
+    c.free()
+    for b in bufs:
+        b.free()
+
+
 def test_attn_all_idle(gpu, xe):
     attn_case(xe, gpu, 14, 4, 1, 256, 16, [0, 0, 0], 2)
 
