@@ -39,7 +39,7 @@ size_t paged_cnt_words();
 // y = act((q . w) s ws + bias) + res over the int8 codes q of norm(x + add)
 // and their row scales s; codes / scales: workspace, rows_q8_codes_bytes() and
 // batch floats.  kp, vec: set by the launch (a row of codes with its padding,
-// whether results go out 16 bytes at a time).
+// whether results of four weight rows go out at once).
 struct RowsQ8 {
   const int8_t *w = nullptr;
   const float *ws = nullptr, *bias = nullptr;

@@ -429,44 +429,82 @@ __global__ __launch_bounds__(64 * KS) void rows_gemm_kernel(RowsQ8 p, int ntile_
   }
 }
 
-// Outputs of NR activation rows x 4 C weight rows whose sums lie in LDS, rows
-// of `stride`: lane l has weight rows r0 + 4 (l % C) .. + 3 of every (64 / C)th
-// activation row.  Four rows' residuals load together.
-template <int ACT, int C, int NR>
+// Outputs of NR activation rows x W C weight rows whose sums lie in LDS, rows
+// of `stride`: lane l has weight rows r0 + W (l % C) .. + W - 1 of every (64 /
+// C)th activation row, so that a row's outputs leave side by side.  The
+// residuals of four or eight rows load together.  ws, bi: of the lane's weight rows.
+template <int ACT, int W, int C, int NR>
 __device__ __forceinline__ void rows_out(const RowsQ8 &p, const int *sums, int stride, int b0, int bj, int r0, const float *sc,
-                                         const f32x4 &ws, const f32x4 &bi) {
-  constexpr int RW = 64 / C, U = NR / RW < 4 ? NR / RW : 4;  // rows a wave has at once
-  const int lane = threadIdx.x & 63, c = 4 * (lane % C), r = r0 + c;
+                                         const float (&ws)[W], const float (&bi)[W]) {
+  constexpr int NO = ACT == XE_ACT_GEGLU ? W / 2 : W;  // outputs of a lane
+  constexpr int RW = 64 / C, M = W == 4 ? 4 : 8, U = NR / RW < M ? NR / RW : M;  // rows at once
+  const int lane = threadIdx.x & 63, c = W * (lane % C), r = r0 + c;
   if (r >= p.m) return;
   const int mo = ACT == XE_ACT_GEGLU ? p.m / 2 : p.m, ro = ACT == XE_ACT_GEGLU ? r / 2 : r;
-  constexpr int NO = ACT == XE_ACT_GEGLU ? 2 : 4;
   typedef float OutV __attribute__((ext_vector_type(NO)));
+  typedef int SumV __attribute__((ext_vector_type(W)));
 #pragma unroll 1
   for (int i0 = lane / C; i0 < NR; i0 += U * RW) {
-    OutV e[U];
+    float e[U][NO];
+    if (p.a.res) {
 #pragma unroll
-    for (int u = 0; u < U; u++)
-      if (p.a.res) e[u] = *reinterpret_cast<const OutV *>(p.a.res + static_cast<size_t>(min(b0 + bj + i0 + u * RW, p.a.batch - 1)) * mo + ro);
+      for (int u = 0; u < U; u++) {
+        const OutV v = *reinterpret_cast<const OutV *>(p.a.res + static_cast<size_t>(min(b0 + bj + i0 + u * RW, p.a.batch - 1)) * mo + ro);
+#pragma unroll
+        for (int i = 0; i < NO; i++) e[u][i] = v[i];
+      }
+#pragma unroll
+      for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int i = 0; i < NO; i++) asm volatile("" : "+v"(e[u][i]));  // none is moved to where it is used
+    }
 #pragma unroll
     for (int u = 0; u < U; u++) {
       const int row = i0 + u * RW, b = b0 + bj + row;
       if (b >= p.a.batch) continue;
-      const i32x4 v = *reinterpret_cast<const i32x4 *>(sums + row * stride + c);
+      const SumV v = *reinterpret_cast<const SumV *>(sums + row * stride + c);
       const float s = sc[bj + row];
-      float z[4];
+      float z[W];
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
+      for (int i = 0; i < W; i++) {
         z[i] = static_cast<float>(v[i]) * s * ws[i];
         if (p.bias) z[i] += bi[i];
       }
       OutV y;
 #pragma unroll
-      for (int i = 0; i < NO; i++) y[i] = ACT == XE_ACT_GEGLU ? gelu_tanh_f(z[2 * i % 4]) * z[2 * i % 4 + 1] : activate(ACT, z[i]);
+      for (int i = 0; i < NO; i++) {
+        if constexpr (ACT == XE_ACT_GEGLU) y[i] = gelu_tanh_f(z[2 * i]) * z[2 * i + 1];
+        else y[i] = activate(ACT, z[i]);
+      }
       if (p.a.res)
 #pragma unroll
         for (int i = 0; i < NO; i++) y[i] += e[u][i];
       *reinterpret_cast<OutV *>(p.a.y + static_cast<size_t>(b) * mo + ro) = y;
     }
+  }
+}
+// The same for all activations: four weight rows a lane where results go out
+// that wide, else one output a lane, up to 64 side by side (512 x 4096 -> 14338 63
+// us with four values a lane one by one, 54 so; 64 x 4096 -> 4098 16.7 and 14.9).
+template <int MW, int NR>
+__device__ __forceinline__ void rows_out_any(const RowsQ8 &p, const int *sums, int stride, int b0, int bj, int r0, const float *sc,
+                                             const float (&ws)[4], const float (&bi)[4]) {
+  if (p.vec) {
+    switch (p.a.act) {
+      case XE_ACT_RELU: return rows_out<XE_ACT_RELU, 4, MW / 4, NR>(p, sums, stride, b0, bj, r0, sc, ws, bi);
+      case XE_ACT_GELU: return rows_out<XE_ACT_GELU, 4, MW / 4, NR>(p, sums, stride, b0, bj, r0, sc, ws, bi);
+      case XE_ACT_SILU: return rows_out<XE_ACT_SILU, 4, MW / 4, NR>(p, sums, stride, b0, bj, r0, sc, ws, bi);
+      case XE_ACT_GEGLU: return rows_out<XE_ACT_GEGLU, 4, MW / 4, NR>(p, sums, stride, b0, bj, r0, sc, ws, bi);
+      default: return rows_out<XE_ACT_NONE, 4, MW / 4, NR>(p, sums, stride, b0, bj, r0, sc, ws, bi);
+    }
+  }
+  const float w1[1] = {ws[0]}, b1[1] = {bi[0]}, w2[2] = {ws[0], ws[1]}, b2[2] = {bi[0], bi[1]};
+  switch (p.a.act) {
+    case XE_ACT_RELU: return rows_out<XE_ACT_RELU, 1, MW, NR>(p, sums, stride, b0, bj, r0, sc, w1, b1);
+    case XE_ACT_GELU: return rows_out<XE_ACT_GELU, 1, MW, NR>(p, sums, stride, b0, bj, r0, sc, w1, b1);
+    case XE_ACT_SILU: return rows_out<XE_ACT_SILU, 1, MW, NR>(p, sums, stride, b0, bj, r0, sc, w1, b1);
+    case XE_ACT_GEGLU: return rows_out<XE_ACT_GEGLU, 2, MW / 2, NR>(p, sums, stride, b0, bj, r0, sc, w2, b2);
+    default: return rows_out<XE_ACT_NONE, 1, MW, NR>(p, sums, stride, b0, bj, r0, sc, w1, b1);
   }
 }
 
@@ -579,12 +617,27 @@ __global__ __launch_bounds__(64 * WV, 2) void rows_tile_kernel(RowsQ8 p, int nti
   issue(1, st[1]);
   // the epilogue's scales: of the tile's activation rows, of a lane's weight rows
   for (int i = tid; i < BN; i += T) sc[i] = b0 + i < p.a.batch ? p.scales[b0 + i] : 0.f;
-  f32x4 ws4 = {0.f, 0.f, 0.f, 0.f}, bi4 = ws4;
+  float ws4[4], bi4[4];
   {
-    const int r = m0 + wm * MW + 4 * (lane % (MW / 4));
-    if (p.vec && r < p.m) {
-      ws4 = *reinterpret_cast<const f32x4 *>(p.ws + r);
-      if (p.bias) bi4 = *reinterpret_cast<const f32x4 *>(p.bias + r);
+    const int each = p.vec ? 4 : p.a.act == XE_ACT_GEGLU ? 2 : 1;  // weight rows of a lane in rows_out
+    const int r = m0 + wm * MW + each * (lane % (MW / each));
+    if (each == 4) {
+      const int r4 = min(r, p.m - 4);
+      const f32x4 w4 = *reinterpret_cast<const f32x4 *>(p.ws + r4);
+      f32x4 b4 = {0.f, 0.f, 0.f, 0.f};
+      if (p.bias) b4 = *reinterpret_cast<const f32x4 *>(p.bias + r4);
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        ws4[i] = w4[i];
+        bi4[i] = b4[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int ri = min(r + min(i, each - 1), p.m - 1);
+        ws4[i] = p.ws[ri];
+        bi4[i] = p.bias ? p.bias[ri] : 0.f;
+      }
     }
   }
   put(0, st[0]);
@@ -634,24 +687,7 @@ __global__ __launch_bounds__(64 * WV, 2) void rows_tile_kernel(RowsQ8 p, int nti
       for (int i = 0; i < FM; i++) *reinterpret_cast<i32x4 *>(out + (16 * j + ln) * RS + 16 * i + 4 * lg) = acc[i][j0 + j];
     __builtin_amdgcn_wave_barrier();
     const int bj = wn * NW + 16 * j0, rj = m0 + wm * MW;
-    if (p.vec) {
-      switch (p.a.act) {
-        case XE_ACT_RELU: rows_out<XE_ACT_RELU, MW / 4, 16 * JH>(p, out, RS, b0, bj, rj, sc, ws4, bi4); break;
-        case XE_ACT_GELU: rows_out<XE_ACT_GELU, MW / 4, 16 * JH>(p, out, RS, b0, bj, rj, sc, ws4, bi4); break;
-        case XE_ACT_SILU: rows_out<XE_ACT_SILU, MW / 4, 16 * JH>(p, out, RS, b0, bj, rj, sc, ws4, bi4); break;
-        case XE_ACT_GEGLU: rows_out<XE_ACT_GEGLU, MW / 4, 16 * JH>(p, out, RS, b0, bj, rj, sc, ws4, bi4); break;
-        default: rows_out<XE_ACT_NONE, MW / 4, 16 * JH>(p, out, RS, b0, bj, rj, sc, ws4, bi4);
-      }
-    } else {
-#pragma unroll 1
-      for (int id = lane; id < 16 * JH * (MW / 4); id += 64) {
-        const int row = id / (MW / 4), c = 4 * (id % (MW / 4));
-        if (b0 + bj + row >= p.a.batch || rj + c >= p.m) continue;
-        Epi4 epi;
-        epi.load(p, b0 + bj + row, rj + c, true);
-        epi.finish(p, b0 + bj + row, rj + c, *reinterpret_cast<const i32x4 *>(out + row * RS + c));
-      }
-    }
+    rows_out_any<MW, 16 * JH>(p, out, RS, b0, bj, rj, sc, ws4, bi4);
     __builtin_amdgcn_wave_barrier();
   }
 }
@@ -717,8 +753,10 @@ int launch_rows_q8(const RowsQ8 &L, hipStream_t s) {
   RowsQ8 r = L;
   r.kp = (r.k + kStep - 1) / kStep * kStep;
   const int outs = r.a.act == XE_ACT_GEGLU ? r.m / 2 : r.m;
-  r.vec = outs % 4 == 0 && ((reinterpret_cast<uintptr_t>(r.a.y) | reinterpret_cast<uintptr_t>(r.a.res) |
-                             reinterpret_cast<uintptr_t>(r.ws) | reinterpret_cast<uintptr_t>(r.bias)) & 15) == 0;
+  // whether results of four weight rows go out at once
+  const uintptr_t rows_at = reinterpret_cast<uintptr_t>(r.a.y) | reinterpret_cast<uintptr_t>(r.a.res) | static_cast<uintptr_t>(outs) * 4;
+  const uintptr_t weights_at = reinterpret_cast<uintptr_t>(r.ws) | reinterpret_cast<uintptr_t>(r.bias);
+  r.vec = ((rows_at & (r.a.act == XE_ACT_GEGLU ? 7 : 15)) | (weights_at & 15)) == 0;
   const bool in16 = ((reinterpret_cast<uintptr_t>(r.a.x) | reinterpret_cast<uintptr_t>(r.a.add) | reinterpret_cast<uintptr_t>(r.a.sum) |
                       reinterpret_cast<uintptr_t>(r.a.post_w)) & 15) == 0;
   // One launch for one row: each workgroup makes the codes for itself, behind its
