@@ -512,11 +512,14 @@ __device__ __forceinline__ void rows_out_any(const RowsQ8 &p, const int *sums, i
 // x BN / 2; K in steps of 128 bytes through two LDS buffers, the loads of two
 // more steps in registers.  Rows lie 128 bytes apart in LDS, their 16-byte
 // chunks permuted by the row, so that 16 rows read together cover all banks.
-// Parts of K as above.  Bound by the
-// matrix instructions: 512 x 4096 -> 14336 in 256 x 128 tiles 41.5 us, 1450 TOP/s on
-// 224 of 256 CUs (a large int8 product reaches 1781 on all).  Smaller tiles by
-// what the CUs load: 200 x 14336 -> 4096 in 64 x 64 tiles and two parts of K 29.8
-// us for 470 MB of operands out of L2, 16 TB/s (runs of 128 bytes reach 17 to 20).
+// Parts of K as above.  Bound by the matrix instructions and the LDS reads that
+// feed them: 512 x 4096 -> 14336 in 256 x 128 tiles 41.0 us, 1470 TOP/s on 224 of
+// 256 CUs with its start and 29 MB of results (such instructions with such reads
+// alone 2650 on all CUs, without reads 3500; a large product of the library 1781).
+// A third LDS buffer, so that reads never follow a barrier: 52.9 us for 52.3 in the
+// whole call.  Smaller tiles by what the CUs load: 200 x 14336 -> 4096 in 64 x 64
+// tiles and two parts of K 29.0 us for 470 MB of operands out of L2, 16 TB/s (runs
+// of 128 bytes reach 17 to 20).
 // Eight waves instead of four, 128 x 64 tiles, 512 x 4096 -> 4096: 28.6 -> 27.3.
 template <int BM, int BN, int WV>
 __global__ __launch_bounds__(64 * WV, 2) void rows_tile_kernel(RowsQ8 p, int ntile_m, int ntile_b, int ksplit) {
