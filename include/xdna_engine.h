@@ -340,7 +340,7 @@ int xe_paged_append_dev(xe_ctx *ctx, const xe_paged_kv *kv,
 /* Attention of one query token a stream over its pages:
  *   q    fp32 [batch, hq * hd] in rows of ldq floats (0: hq * hd)
  *   lens int32 [batch]: tokens of the stream, the new one included
- *   out  fp32 [batch, hq * hd] in rows of ldo floats (0: hq * hd)
+ *   out  fp32 [batch, hq * hd] in rows of ldo floats (0: hq * hd); may be q
  * scores = (q . k) * scale; softmax over the positions [0, lens[b]), with
  * window > 0 over the last `window` of them, of which the table has the page.
  * Query head h reads kv head h / (hq / hkv); hq is a multiple of hkv.  A
@@ -369,8 +369,9 @@ typedef struct xe_w8a8_rows {
   const float *post_w; /* [k]: add goes through RMSNorm (1 + w) first, with
                           post_eps (Gemma's post norms), or null */
   float *sum;          /* [batch, k] receives x + add, or null; may be x or add */
-  const float *res;    /* [batch, outputs] added after the activation, or null */
-  float *y;            /* [batch, outputs]; may be res */
+  const float *res;    /* [batch, outputs] added after the activation, or null;
+                          may be x or sum */
+  float *y;            /* [batch, outputs]; may be res, x, add or sum */
   int batch;           /* 1..512 */
   int act;             /* enum xe_act */
   float post_eps;      /* read with post_w alone */

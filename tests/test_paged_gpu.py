@@ -305,6 +305,25 @@ def test_attn_one_long_stream_among_short_ones(gpu, xe, hq, hkv, hd):
         b.free()
 
 
+@pytest.mark.parametrize("hq,hkv,hd,lens", [(4, 1, 256, [3000, 0, 17]), (20, 1, 128, [700]), (2, 1, 64, list(range(0, 700, 10)))])
+def test_attn_over_its_queries(gpu, xe, hq, hkv, hd, lens):
+    dev, ctx = gpu
+    rng = np.random.default_rng(len(lens))
+    c = Cache(xe, dev, rng, len(lens), -(-max(lens) // 16), 16, hkv, hd)
+    kv = c.upload()
+    q = rng.standard_normal((len(lens), hq, hd)).astype(np.float32)
+    bufs = [put(xe, dev, a) for a in (q, np.array(lens, np.int32), q)]
+    ctx.paged_attn_dev(kv, bufs[0], bufs[1], hq, 0.1, bufs[0])
+    ctx.paged_attn_dev(kv, bufs[2], bufs[1], hq, 0.1, bufs[2])
+    ctx.synchronize()
+    want, bound = attn64(c, q, lens, hq, 0.1)
+    for b in (bufs[0], bufs[2]):
+        within(b.read(np.float32, q.size).reshape(q.shape), want, bound, "over the queries")
+    c.free()
+    for b in bufs:
+        b.free()
+
+
 def test_attn_all_idle(gpu, xe):
     attn_case(xe, gpu, 14, 4, 1, 256, 16, [0, 0, 0], 2)
 

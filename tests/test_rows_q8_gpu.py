@@ -100,6 +100,35 @@ def test_aliases(gpu, xe, alias):
         rows_case(xe, gpu, 130, 272, batch, norm=2, add=True, res=True, alias=alias)
 
 
+@pytest.mark.parametrize("batch", [1, 2, 30, 140])
+@pytest.mark.parametrize("what", ["y is res is x", "res is sum", "sum is y", "y is add"])
+def test_residual_stream_in_place(gpu, xe, batch, what):
+    """The stream that a layer adds to, read and written by one call."""
+    dev, ctx = gpu
+    rng = np.random.default_rng(batch)
+    n = 272
+    w, defs = make_weight(xe, ctx, rng, n, n, True, 2)
+    x, a = (rng.standard_normal((batch, n)).astype(np.float32) for _ in range(2))
+    bx, ba, by, bs = (put(xe, dev, v) for v in (x, a, np.zeros_like(x), np.zeros_like(x)))
+    if what == "y is res is x":
+        ctx.w8a8_rows_dev(w, xe.W8a8Rows(batch, bx.ptr, bx.ptr, res=bx.ptr))
+        want, _, bound = rows64(*defs, x, res=x)
+        got = bx
+    elif what == "res is sum":
+        ctx.w8a8_rows_dev(w, xe.W8a8Rows(batch, bx.ptr, by.ptr, add=ba.ptr, sum=bs.ptr, res=bs.ptr))
+        want, _, bound = rows64(*defs, x, a, res=x + a)
+        got = by
+    else:
+        got = by if what == "sum is y" else ba
+        ctx.w8a8_rows_dev(w, xe.W8a8Rows(batch, bx.ptr, got.ptr, add=ba.ptr, sum=by.ptr))
+        want, _, bound = rows64(*defs, x, a)
+    ctx.synchronize()
+    within(got.read(np.float32, batch * n).reshape(batch, n), want, bound, what)
+    w.free()
+    for b in (bx, ba, by, bs):
+        b.free()
+
+
 def test_rows_do_not_depend_on_each_other(gpu, xe):
     """A row's result is the same alone and beside rows a thousand times larger,
     at every batch (kernels change with it)."""
@@ -184,7 +213,13 @@ def test_refusals_over_weights(gpu, xe):
     for w, act in ((odd, xe.XE_ACT_GEGLU), (wide, 0), (half, 0), (tilted, 0)):
         with pytest.raises(xe.XdnaError):
             ctx.w8a8_rows_dev(w, xe.W8a8Rows(1, b.ptr, b.ptr, act=act))
-    for w in (odd, wide, half, tilted):
+    broken = ctx.register_weight_q8(np.ones((4, 16), np.int8), np.ones(4, np.float32))
+    for norm, gamma in ((2, None), (1, np.ones(16, np.float32))):  # a norm that was refused
+        with pytest.raises(xe.XdnaError):
+            ctx.set_norm(broken, xe.Norm(norm, gamma, None, 1e-6))
+        with pytest.raises(xe.XdnaError):
+            ctx.w8a8_rows_dev(broken, xe.W8a8Rows(1, b.ptr, b.ptr))
+    for w in (odd, wide, half, tilted, broken):
         w.free()
     b.free()
 
