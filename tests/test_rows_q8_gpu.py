@@ -68,6 +68,14 @@ def test_shapes(gpu, xe, m, k, batch):
     rows_case(xe, gpu, m, k, batch, norm=1, seed=5)
 
 
+@pytest.mark.parametrize("m", [3, 4096, 4112])
+@pytest.mark.parametrize("k", [16, 768, 784, 1280, 1296])
+def test_few_rows(gpu, xe, m, k):
+    """One launch and two, at the sizes where they change."""
+    for batch in (1, 2, 7, 8, 9):
+        rows_case(xe, gpu, m, k, batch, norm=1 + batch % 3, act=3, add=True, post=batch > 2, res=True, seed=3)
+
+
 @pytest.mark.parametrize("m,k,batch", [(301, 720, 509), (702, 160, 511), (702, 4112, 397), (702, 8208, 197), (2102, 304, 509),
                                        (4102, 1040, 510), (8200, 8208, 449), (14402, 4112, 400), (97, 8208, 5),
                                        (97, 8208, 200)])

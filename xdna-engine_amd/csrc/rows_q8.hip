@@ -22,6 +22,8 @@ constexpr size_t kPartBytes = rowsform::kPartBytes;  // partial tiles of K split
 constexpr size_t kCntWords = rowsform::kTiles;       // and their arrival counters
 constexpr int kMaxSplit = 4;        // parts of K
 constexpr int kStep = 128;          // bytes of K a step
+constexpr int kManyRows = 8;       // rows that its eight waves make, one each
+constexpr int kManyK = 1280;       // K up to which they do
 constexpr int kFusedK = 4096;       // K up to which a workgroup makes one row's codes itself
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -56,8 +58,8 @@ __device__ __forceinline__ double other64(double v) {
     return (threadIdx.x & (HALF ? 32 : 16)) ? r[0] : r[1];
   });
 }
-// op over all threads of the workgroup, the same in each; red: T / 64 doubles
-// of a slot that no wave still reads.
+// op over all T threads of the workgroup, or over the wave (T = 64), the same in
+// each; red: T / 64 doubles of a slot that no wave still reads (T = 64: none).
 template <int T, typename Op>
 __device__ __forceinline__ double block_all(double v, double *red, Op op) {
   v = op(v, dpp64<gdev::kDppXor1>(v));
@@ -66,6 +68,7 @@ __device__ __forceinline__ double block_all(double v, double *red, Op op) {
   v = op(v, dpp64<gdev::kDppMirror>(v));
   v = op(v, other64<false>(v));
   v = op(v, other64<true>(v));
+  if constexpr (T == 64) return v;
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
   v = red[0];
@@ -98,10 +101,10 @@ __device__ __forceinline__ size_t code_at(const RowsQ8 &p, int b, int i) {
 
 // Row b to codes by T threads, a thread holding elements 4 (tid + T j) .. + 3:
 // put(i, four codes) for each four below kp, the scale returned.  `sum` is
-// written where `writes`.  red: four slots, not those of the row before.
+// written where `writes`.  red: four slots of T / 64 (T = 64: none).
 template <int NV, int T, bool VEC, typename Put>
-__device__ __forceinline__ float quant_row(const RowsQ8 &p, int b, bool writes, double (*red)[T / 64], Put &&put) {
-  const int K = p.k, tid = threadIdx.x;
+__device__ __forceinline__ float quant_row(const RowsQ8 &p, int b, bool writes, double *red, Put &&put) {
+  const int K = p.k, tid = threadIdx.x % T;
   const size_t at = static_cast<size_t>(b) * K;
   // All loads of the row in flight at once where 4 waves a SIMD leave registers
   // for them (128 each), otherwise the norms' where they are used.
@@ -124,7 +127,7 @@ __device__ __forceinline__ float quant_row(const RowsQ8 &p, int b, bool writes, 
 #pragma unroll
       for (int c = 0; c < 4; c++)
         if (4 * (tid + T * j) < K) v = __builtin_fma(static_cast<double>(su[j][c]), static_cast<double>(su[j][c]), v);
-    const double inv = 1.0 / sqrt(block_all<T>(v, red[0], Sum64{}) / K + static_cast<double>(p.a.post_eps));
+    const double inv = 1.0 / sqrt(block_all<T>(v, red + 0 * (T / 64), Sum64{}) / K + static_cast<double>(p.a.post_eps));
 #pragma unroll
     for (int j = 0; j < NV; j++)
 #pragma unroll
@@ -159,7 +162,7 @@ __device__ __forceinline__ float quant_row(const RowsQ8 &p, int b, bool writes, 
       for (int j = 0; j < NV; j++)
 #pragma unroll
         for (int c = 0; c < 4; c++) v += h[j][c];
-      const double mean = block_all<T>(v, red[1], Sum64{}) / K;
+      const double mean = block_all<T>(v, red + 1 * (T / 64), Sum64{}) / K;
       v = 0.0;
 #pragma unroll
       for (int j = 0; j < NV; j++)
@@ -170,7 +173,7 @@ __device__ __forceinline__ float quant_row(const RowsQ8 &p, int b, bool writes, 
     for (int j = 0; j < NV; j++)
 #pragma unroll
       for (int c = 0; c < 4; c++) v = __builtin_fma(h[j][c], h[j][c], v);
-    const double inv = 1.0 / sqrt(block_all<T>(v, red[2], Sum64{}) / K + static_cast<double>(p.eps));
+    const double inv = 1.0 / sqrt(block_all<T>(v, red + 2 * (T / 64), Sum64{}) / K + static_cast<double>(p.eps));
     const double one = p.norm == XE_NORM_RMS1P ? 1.0 : 0.0;
 #pragma unroll
     for (int j = 0; j < NV; j++)
@@ -192,7 +195,7 @@ __device__ __forceinline__ float quant_row(const RowsQ8 &p, int b, bool writes, 
       a = fmax(a, fabs(h[j][c]));
       bad = __builtin_fma(h[j][c], 0.0, bad);
     }
-  const double amax = block_all<T>(bad == 0.0 ? a : INFINITY, red[3], Max64{});
+  const double amax = block_all<T>(bad == 0.0 ? a : INFINITY, red + 3 * (T / 64), Max64{});
   float s = static_cast<float>(amax / 127.0);
   if (!(s > 0.f)) s = 1.f;
   const bool number = s < INFINITY;  // else NaN or infinity in the row: its scale, and its outputs, become NaN
@@ -221,7 +224,7 @@ __device__ __forceinline__ float quant_row(const RowsQ8 &p, int b, bool writes, 
 // threads: 300 of 8192 0.7 more.  K beyond 16384 spills 90 registers.
 template <int NV, int T, bool VEC>
 __global__ __launch_bounds__(T) void rows_quant_kernel(RowsQ8 p) {
-  __shared__ double red[4][T / 64];
+  __shared__ double red[4 * (T / 64)];
   const int b = blockIdx.x;
   const float s = quant_row<NV, T, VEC>(p, b, true, red, [&](int i, uint32_t q) {
     *reinterpret_cast<uint32_t *>(p.codes + code_at(p, b, i)) = q;
@@ -312,22 +315,24 @@ struct Epi4 {
 // Tiles of WR x 16 weight rows and NJ x 16 activation rows a workgroup, its KS
 // waves each over their own part of K (v_mfma_i32_16x16x64_i8: a lane holds 16
 // consecutive k of weight row lane % 16 and of activation row lane % 16), U
-// steps of 64 in flight.  NV > 0: the workgroup makes the codes itself (K <= 1024
-// NV, one row), into LDS, while its first weights load.  Bound by the weights'
+// steps of 64 in flight.  NV > 0: the workgroup makes the codes itself, into LDS,
+// while its first weights load: one row (K <= 1024 NV), or (MANY) a row a wave (K
+// <= 256 NV).  Bound by the weights'
 // way to the CUs: 64 x 4096 -> 4096 7.3 us for 17 MB of weights (3.5 at a large
 // copy's 4.86 TB/s) that two tiles of rows each read; one row 1152 -> 13824 6.4 for
 // 16 MB.  The waves' sums meet in LDS.  A CU draws such rows of 64 bytes at 37 B/ns,
 // so that few tiles of a long K are bound by that: parts of K (ksplit) go to
 // other CUs then and leave their sums in `part`; the last workgroup of a tile to
 // arrive adds them, integers, so that their order changes nothing.
-template <int WR, int NJ, int KS, int U, int NV>
+template <int WR, int NJ, int KS, int U, int NV, bool MANY>
 __global__ __launch_bounds__(64 * KS) void rows_gemm_kernel(RowsQ8 p, int ntile_m, int ntile_b, int ksplit) {
   constexpr int NB = WR * NJ;                     // 16 x 16 blocks
   constexpr bool kFused = NV > 0;
-  static_assert(!kFused || (KS == 4 && NJ == 1), "one row made here by 256 threads");
+  static_assert(!kFused || (KS == (MANY ? 8 : 4) && NJ == 1), "one row by 256 threads, or a row a wave");
   __shared__ __attribute__((aligned(16))) int part[KS][NB][256];
-  __shared__ __attribute__((aligned(16))) int8_t codes[kFused ? kFusedK : 16];
-  __shared__ double red[kFused ? 4 : 1][4];
+  __shared__ __attribute__((aligned(16))) int8_t codes[MANY ? 256 * 16 * NV : kFused ? kFusedK : 16];
+  __shared__ double red[kFused && !MANY ? 16 : 1];
+  __shared__ float made[16];
   __shared__ int flag;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 15, lg = lane >> 4;
@@ -370,14 +375,22 @@ __global__ __launch_bounds__(64 * KS) void rows_gemm_kernel(RowsQ8 p, int ntile_
   const int ob = b0 + 16 * (wave % NJ) + ln, orow = r0 + 16 * (wave / NJ) + 4 * lg;
   Epi4 epi;
   if (wave < NB) epi.load(p, ob, orow, !kFused);
-  if constexpr (kFused) {
+  if constexpr (MANY) {
+    const float s = quant_row<NV, 64, true>(p, min(wave, p.a.batch - 1), tm == 0 && wave < p.a.batch, nullptr, [&](int i, uint32_t c) {
+      *reinterpret_cast<uint32_t *>(codes + ((i / 64 * 4 + i % 64 / 16) * 16 + wave) * 16 + i % 16) = c;
+    });
+    if (lane == 0) made[wave] = s;
+    __syncthreads();
+    epi.s = made[ln];
+  } else if constexpr (kFused) {
     epi.s = quant_row<NV, 256, true>(p, 0, at == 0, red, [&](int i, uint32_t c) { *reinterpret_cast<uint32_t *>(codes + i) = c; });
     __syncthreads();
   }
   for (int s = s0; s < s1; s += U) {
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      if constexpr (kFused) x[u][0] = *reinterpret_cast<const i32x4 *>(codes + min(64 * (s + u), kp - 64) + 16 * lg);
+      if constexpr (MANY) x[u][0] = *reinterpret_cast<const i32x4 *>(codes + min(s + u, kp / 64 - 1) * 1024 + 16 * lane);
+      else if constexpr (kFused) x[u][0] = *reinterpret_cast<const i32x4 *>(codes + min(64 * (s + u), kp - 64) + 16 * lg);
 #pragma unroll
       for (int r = 0; r < WR; r++)
 #pragma unroll
@@ -704,12 +717,12 @@ void check_tiles(int tm, int tb, int ksplit, int bm, int bn) {
              "rows gemm: partial tiles beyond the workspace");
 }
 
-template <int WR, int NJ, int KS, int U, int NV = 0>
+template <int WR, int NJ, int KS, int U, int NV = 0, bool MANY = false>
 void launch_gemm(const RowsQ8 &r, int ksplit, hipStream_t s) {
   const int tm = (r.m + 16 * WR - 1) / (16 * WR), tb = (r.a.batch + 16 * NJ - 1) / (16 * NJ);
   check_tiles(tm, tb, ksplit, 16 * WR, 16 * NJ);
   const int blocks = (tm * tb * ksplit + kXcds - 1) / kXcds * kXcds;
-  hipLaunchKernelGGL((rows_gemm_kernel<WR, NJ, KS, U, NV>), dim3(blocks), dim3(64 * KS), 0, s, r, tm, tb, ksplit);
+  hipLaunchKernelGGL((rows_gemm_kernel<WR, NJ, KS, U, NV, MANY>), dim3(blocks), dim3(64 * KS), 0, s, r, tm, tb, ksplit);
   XE_HIP(hipGetLastError());
 }
 
@@ -772,6 +785,16 @@ int launch_rows_q8(const RowsQ8 &L, hipStream_t s) {
     if (r.k <= 1024) wide ? launch_gemm<2, 1, 4, 4, 1>(r, 1, s) : launch_gemm<1, 1, 4, 8, 1>(r, 1, s);
     else if (r.k <= 2048) wide ? launch_gemm<2, 1, 4, 4, 2>(r, 1, s) : launch_gemm<1, 1, 4, 8, 2>(r, 1, s);
     else wide ? launch_gemm<2, 1, 4, 4, 4>(r, 1, s) : launch_gemm<1, 1, 4, 8, 4>(r, 1, s);
+    return 1;
+  }
+  // Up to eight rows, a wave each, where that is one tile a CU.  us in one launch /
+  // in two, 2 and 8 rows: 768 -> 1536 5.4 / 6.8, 5.4 / 6.9, 1152 -> 4096 6.6 / 7.1,
+  // 6.6 / 7.4; 1600 -> 4096 7.6 / 7.1, 7.4 / 7.3; 16 rows on four waves of two
+  // halves, twice, 768 -> 1536 8.4 / 6.4; 1152 -> 13824 20 / 8.8.  One row so:
+  // 768 -> 1536 5.3, on all its workgroup's threads 4.6.
+  if (in16 && r.a.batch <= kManyRows && r.m <= 16 * gdev::cu_count() && r.k <= kManyK && !shares(r, outs)) {
+    if (r.k <= 768) launch_gemm<1, 1, 8, 2, 3, true>(r, 1, s);
+    else launch_gemm<1, 1, 8, 3, 5, true>(r, 1, s);
     return 1;
   }
   if (in16) launch_quant<true>(r, s);
