@@ -318,8 +318,8 @@ struct Epi4 {
 // steps of 64 in flight.  NV > 0: the workgroup makes the codes itself, into LDS,
 // while its first weights load: one row (K <= 1024 NV), or (MANY) a row a wave (K
 // <= 256 NV).  Bound by the weights'
-// way to the CUs: 64 x 4096 -> 4096 7.3 us for 17 MB of weights (3.5 at a large
-// copy's 4.86 TB/s) that two tiles of rows each read; one row 1152 -> 13824 6.4 for
+// way to the CUs: 64 x 4096 -> 4096 8.4 us for 17 MB of weights (3.5 at a large
+// copy's 4.86 TB/s) that two tiles of rows each read; one row 1152 -> 13824 7.4 for
 // 16 MB.  The waves' sums meet in LDS.  A CU draws such rows of 64 bytes at 37 B/ns,
 // so that few tiles of a long K are bound by that: parts of K (ksplit) go to
 // other CUs then and leave their sums in `part`; the last workgroup of a tile to
@@ -789,8 +789,8 @@ int launch_rows_q8(const RowsQ8 &L, hipStream_t s) {
   }
   // Up to eight rows, a wave each, where that is one tile a CU.  us in one launch /
   // in two, 2 and 8 rows: 768 -> 1536 5.4 / 6.8, 5.4 / 6.9, 1152 -> 4096 6.6 / 7.1,
-  // 6.6 / 7.4; 1600 -> 4096 7.6 / 7.1, 7.4 / 7.3; 16 rows on four waves of two
-  // halves, twice, 768 -> 1536 8.4 / 6.4; 1152 -> 13824 20 / 8.8.  One row so:
+  // 6.6 / 7.4; 1600 -> 4096 7.6 / 7.1, 7.4 / 7.3; 16 rows on sixteen waves 768 ->
+  // 1536 7.0 / 6.4, 256 -> 1536 6.4 / 6.2; tiles for four CUs 1152 -> 13824 20 / 8.8.  One row so:
   // 768 -> 1536 5.3, on all its workgroup's threads 4.6.
   if (in16 && r.a.batch <= kManyRows && r.m <= 16 * gdev::cu_count() && r.k <= kManyK && !shares(r, outs)) {
     if (r.k <= 768) launch_gemm<1, 1, 8, 2, 3, true>(r, 1, s);
