@@ -790,8 +790,8 @@ int launch_rows_q8(const RowsQ8 &L, hipStream_t s) {
   // Up to eight rows, a wave each, where that is one tile a CU.  us in one launch /
   // in two, 2 and 8 rows: 768 -> 1536 5.4 / 6.8, 5.4 / 6.9, 1152 -> 4096 6.6 / 7.1,
   // 6.6 / 7.4; 1600 -> 4096 7.6 / 7.1, 7.4 / 7.3; 16 rows on sixteen waves 768 ->
-  // 1536 7.0 / 6.4, 256 -> 1536 6.4 / 6.2; tiles for four CUs 1152 -> 13824 20 / 8.8.  One row so:
-  // 768 -> 1536 5.3, on all its workgroup's threads 4.6.
+  // 1536 7.0 / 6.4, 256 -> 1536 6.4 / 6.2; four tiles a CU, 1152 -> 13824, 20 / 8.8.
+  // One row so: 768 -> 1536 5.3, on all its workgroup's threads 4.6.
   if (in16 && r.a.batch <= kManyRows && r.m <= 16 * gdev::cu_count() && r.k <= kManyK && !shares(r, outs)) {
     if (r.k <= 768) launch_gemm<1, 1, 8, 2, 3, true>(r, 1, s);
     else launch_gemm<1, 1, 8, 3, 5, true>(r, 1, s);
