@@ -346,9 +346,11 @@ int xe_paged_append_dev(xe_ctx *ctx, const xe_paged_kv *kv,
  * Query head h reads kv head h / (hq / hkv); hq is a multiple of hkv.  A
  * stream with no such position (lens[b] <= 0: an idle slot) gets zeros;
  * positions beyond the table hold no keys.  Keys and values outside the
- * range, in the same page too, are never used whatever they hold; a value in
- * the range that is not finite leaves its dimension not finite.  Results do
- * not change from call to call. */
+ * range, in the same page too, are never used whatever they hold.  In the
+ * range, a value that is not finite leaves its dimension not finite; a query
+ * that is not finite makes its head NaN, a key that is NaN the heads that read
+ * it; an infinite key makes them NaN too, or, where its score is -infinity,
+ * has no weight.  Results do not change from call to call. */
 int xe_paged_attn_dev(xe_ctx *ctx, const xe_paged_kv *kv, const float *q_dev,
                       uint64_t ldq, const int32_t *lens_dev, int hq,
                       float scale, int window, float *out_dev, uint64_t ldo);

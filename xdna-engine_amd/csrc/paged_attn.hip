@@ -524,11 +524,12 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(Params p) {
           for (int k = 0; k < kGroup; k++) mx = fmaxf(mx, mk[k]);
 #pragma unroll
           for (int k = 0; k < kGroup; k++) {
-            const bool none = mk[k] == -INFINITY || k >= static_cast<int>(cnt);
-            const float f = none ? 0.f : __builtin_amdgcn_exp2f(mk[k] - mx);
-            ls += none ? 0.f : lk[k] * f;
+            // A partial without keys holds zeros; one whose scores are all NaN
+            // has no maximum either, and its sums have to stay in.
+            const float f = mk[k] == -INFINITY || k >= static_cast<int>(cnt) ? 0.f : __builtin_amdgcn_exp2f(mk[k] - mx);
+            ls += lk[k] * f;
 #pragma unroll
-            for (int z = 0; z < 4; z++) x[z] += none ? 0.f : v[k][z] * f;
+            for (int z = 0; z < 4; z++) x[z] += v[k][z] * f;
           }
           if (final) {
             finish(i, x, ls);
