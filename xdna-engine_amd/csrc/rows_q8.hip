@@ -99,6 +99,12 @@ __device__ __forceinline__ size_t code_at(const RowsQ8 &p, int b, int i) {
   return ((static_cast<size_t>(i / 64) * row_groups(p.a.batch) + b / 16) * 64 + i % 64 / 16 * 16 + b % 16) * 16 + i % 16;
 }
 
+// h / s is taken as h r with r = 1 / s, within 2^-46 of it for codes up to 127, so
+// a half may come out just below one: 2^-44 more than a half lifts it.  The
+// quotient of two fp32 values that is no half is 2^-26 or more away from one;
+// behind a norm h itself is known to about 2^-44.
+constexpr double kHalf = 0.5 + 0x1p-44;
+
 // Row b to codes by T threads, a thread holding elements 4 (tid + T j) .. + 3:
 // put(i, four codes) for each four below kp, the scale returned.  `sum` is
 // written where `writes`.  red: four slots of T / 64 (T = 64: none).
@@ -207,7 +213,7 @@ __device__ __forceinline__ float quant_row(const RowsQ8 &p, int b, bool writes, 
     uint32_t q = 0;
 #pragma unroll
     for (int c = 0; c < 4; c++) {  // half a unit away from zero, then cut; a scale below fp32's normal range may leave more than 127
-      const int code = static_cast<int>(__builtin_fma(h[j][c], r, copysign(0.5, h[j][c])));
+      const int code = static_cast<int>(__builtin_fma(h[j][c], r, copysign(kHalf, h[j][c])));
       q |= (static_cast<uint32_t>(min(max(code, -127), 127)) & 0xffu) << (8 * c);
     }
     put(i, number && i < K ? q : 0u);
