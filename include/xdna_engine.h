@@ -313,7 +313,8 @@ typedef struct xe_paged_rows {
                                queries), k and v [n_rows, hkv * hd] in rows of
                                ldkv: the parts of a fused projection's rows */
   uint64_t ldq, ldkv;       /* floats from row to row */
-  float *q_out;             /* [n_rows, hq * hd] in rows of ldqo; may be q */
+  float *q_out;             /* [n_rows, hq * hd] in rows of ldqo; may be q, with
+                               the same stride */
   uint64_t ldqo;
   const int32_t *pos;       /* [batch] */
   const int32_t *start;     /* [batch + 1], ascending, or null */
@@ -340,7 +341,8 @@ int xe_paged_append_dev(xe_ctx *ctx, const xe_paged_kv *kv,
 /* Attention of one query token a stream over its pages:
  *   q    fp32 [batch, hq * hd] in rows of ldq floats (0: hq * hd)
  *   lens int32 [batch]: tokens of the stream, the new one included
- *   out  fp32 [batch, hq * hd] in rows of ldo floats (0: hq * hd); may be q
+ *   out  fp32 [batch, hq * hd] in rows of ldo floats (0: hq * hd); may be q,
+ *        with the same stride (another is refused for more than one stream)
  * scores = (q . k) * scale; softmax over the positions [0, lens[b]), with
  * window > 0 over the last `window` of them, of which the table has the page.
  * Query head h reads kv head h / (hq / hkv); hq is a multiple of hkv.  A

@@ -1124,6 +1124,7 @@ int xe_paged_attn_dev(xe_ctx *ctx, const xe_paged_kv *kv, const float *q_dev, ui
     a.out = out_dev;
     a.ldo = ldo ? ldo : qw;
     XE_REQUIRE(a.ldq >= qw && a.ldq <= most && a.ldo >= qw && a.ldo <= most, "paged attention: ldq or ldo below hq * hd");
+    XE_REQUIRE(out_dev != q_dev || a.ldo == a.ldq || a.kv.batch == 1, "paged attention: out over q needs its row stride");
     XE_REQUIRE(window >= 0, "paged attention: window must not be negative");
     XE_REQUIRE(std::isfinite(scale), "paged attention: scale must be finite");
     XE_REQUIRE(ctx, "null ctx");
