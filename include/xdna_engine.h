@@ -178,7 +178,9 @@ xe_weight *xe_register_fused(xe_ctx *ctx, int wdtype, int m, int k,
                              const float *w, int layout, int norm,
                              const float *gamma, const float *beta, float eps,
                              const float *bias);
-/* Attach a pre-norm to an already registered weight (q8/bfp16/bf16). */
+/* Attach a pre-norm to an already registered weight (q8/bfp16/bf16).  Where
+ * gamma or beta is missing or cannot be copied, the call fails, and every call
+ * that applies the weight's norm is refused until one is set. */
 int xe_weight_set_norm(xe_weight *w, int norm, const float *gamma,
                        const float *beta, float eps);
 void xe_weight_free(xe_weight *w);

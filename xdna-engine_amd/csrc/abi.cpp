@@ -263,7 +263,15 @@ void set_norm(xe_weight *w, int norm, const float *gamma, const float *beta, flo
   }
 }
 
+// A norm that was refused, or that could not be copied, leaves the weight without
+// its gamma or beta: no call applies it.
+void require_norm(const xe_weight *w) {
+  XE_REQUIRE((w->norm == XE_NORM_NONE || w->gamma) && (w->norm != XE_NORM_LN || w->beta),
+             "the weight's norm lacks gamma or beta");
+}
+
 GemvLaunch gemv_args(const xe_weight *w, const void *x, int x_dtype, int batch, float *y) {
+  require_norm(w);
   GemvLaunch g;
   g.wdtype = w->wdtype;
   g.w = w->w;
@@ -1148,7 +1156,7 @@ int xe_w8a8_rows_dev(xe_ctx *ctx, const xe_weight *w, const xe_w8a8_rows *rows) 
     XE_REQUIRE(w->k <= 32768, "xe_w8a8_rows: K beyond 32768");
     XE_REQUIRE(static_cast<size_t>(w->m) * w->k < (size_t(1) << 31), "xe_w8a8_rows: weight above 2 GB");
     XE_REQUIRE((reinterpret_cast<uintptr_t>(w->w) & 15) == 0, "xe_w8a8_rows: weight view off a multiple of 16 bytes");
-    XE_REQUIRE((w->norm == XE_NORM_NONE || w->gamma) && (w->norm != XE_NORM_LN || w->beta), "xe_w8a8_rows: the weight's norm lacks gamma or beta");
+    require_norm(w);
     DeviceGuard dg(ctx->dev->ordinal);
     RowsQ8 r;
     r.w = static_cast<const int8_t *>(w->w);
