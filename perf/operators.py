@@ -9,6 +9,11 @@
 
 `run` computes them in plain torch, or, where `own` is true, through the
 library; `exact` restates them in 64 bits.
+
+The library's calls queue on a stream of their own, which neither waits for
+torch's streams nor makes them wait: `prepare` ends when its inputs are there,
+and what `run` returns is there once the device has been waited for
+(`torch.cuda.synchronize()`, or the context's `synchronize()`).
 """
 import math
 import os
@@ -249,7 +254,11 @@ def _handles(st):
 
 def prepare(case, seed):
     st = {"append": _prepare_append, "attn": _prepare_attn, "rows": _prepare_rows}[case["kind"]](case, seed)
-    return _handles(st) if own else st
+    if not own:
+        return st
+    st = _handles(st)
+    torch.cuda.synchronize()  # the library's stream does not wait for torch's
+    return st
 
 
 # ---------------------------------------------------------------------------
