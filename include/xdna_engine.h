@@ -327,7 +327,8 @@ typedef struct xe_paged_rows {
                                the position; null: no rotation */
   float eps;
   int rope_len;
-  int n_rows, hq;           /* hq is not read without q */
+  int n_rows, hq;           /* hq is not read without q; n_rows * (hq + 2 hkv) * hd
+                               < 2^35 - 2048 */
 } xe_paged_rows;
 
 /* Appends rows to the streams' pages, keys and values rounded to bf16 (RNE),
@@ -347,7 +348,9 @@ int xe_paged_append_dev(xe_ctx *ctx, const xe_paged_kv *kv,
  *        with the same stride (another is refused for more than one stream)
  * scores = (q . k) * scale; softmax over the positions [0, lens[b]), with
  * window > 0 over the last `window` of them, of which the table has the page.
- * Query head h reads kv head h / (hq / hkv); hq is a multiple of hkv.  A
+ * Query head h reads kv head h / (hq / hkv); hq is a multiple of hkv, and
+ * batch * hkv * ceil(hq / hkv / 16) times the table's max_pages * page_size
+ * positions stay below 2^35.  A
  * stream with no such position (lens[b] <= 0: an idle slot) gets zeros;
  * positions beyond the table hold no keys.  Keys and values outside the
  * range, in the same page too, are never used whatever they hold.  In the

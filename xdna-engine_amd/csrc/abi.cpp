@@ -1107,6 +1107,8 @@ int xe_paged_append_dev(xe_ctx *ctx, const xe_paged_kv *kv, const xe_paged_rows 
     XE_REQUIRE(!r.rope_cos == !r.rope_sin, "paged append: one of rope_cos and rope_sin");
     XE_REQUIRE(!r.rope_cos || r.rope_len >= 1, "paged append: rope_len must be positive");
     XE_REQUIRE((!r.q_norm_w && !r.k_norm_w) || r.eps >= 0.f, "paged append: eps must not be negative");
+    XE_REQUIRE(static_cast<int64_t>(r.n_rows) * (r.hq + 2 * v.hkv) * v.hd < (int64_t(1) << 35) - 2048,
+               "paged append: more rows than one call takes");
     XE_REQUIRE(ctx, "null ctx");
     DeviceGuard dg(ctx->dev->ordinal);
     launch_paged_append(v, r, ctx->dev->stream);
@@ -1134,6 +1136,10 @@ int xe_paged_attn_dev(xe_ctx *ctx, const xe_paged_kv *kv, const float *q_dev, ui
     XE_REQUIRE(a.ldq >= qw && a.ldq <= most && a.ldo >= qw && a.ldo <= most, "paged attention: ldq or ldo below hq * hd");
     XE_REQUIRE(out_dev != q_dev || a.ldo == a.ldq || a.kv.batch == 1, "paged attention: out over q needs its row stride");
     XE_REQUIRE(window >= 0, "paged attention: window must not be negative");
+    // blocks of 16 keys are counted in 32 bits
+    const int64_t keys = static_cast<int64_t>(kv->max_pages) * kv->page_size;
+    XE_REQUIRE(keys / 16 * a.kv.batch * a.kv.hkv * ((hq / a.kv.hkv + 15) / 16) < (int64_t(1) << 31),
+               "paged attention: more keys in the table than one call takes");
     XE_REQUIRE(std::isfinite(scale), "paged attention: scale must be finite");
     XE_REQUIRE(ctx, "null ctx");
     DeviceGuard dg(ctx->dev->ordinal);
