@@ -47,19 +47,11 @@ constexpr int kRows = 16;    // query heads a unit at most
 constexpr int kMaxWg = 512;
 constexpr int kGroup = 16;   // partials merged at once
 constexpr int kMaxHd = 256;
-// Two forms.  Workgroups of eight waves, one a CU, whole ones a unit, so that a
-// workgroup has one unit's chain of loads before it: up to 64 streams of up to
-// a unit a CU, of fewer than kManyUnits units or of keys (those the table or
-// the window allows) up to kFewBytes.  Else of four waves, two a CU, in equal
-// shares of all keys, with nontemporal loads.  us with the first / the second:
-// 32768 keys of one stream (4 x 256) 18.2 / 23.6, 8 mixed streams to 3000 keys
-// (8 / 2 x 128) 9.7 / 10.8, 32 of window 1024 12.5 / 16.5, 60 to 300 keys (16 /
-// 4 x 128) 9.4 / 13.6, 64 to 1500 (4 x 256) 20.9 / 26.5, 64 to 4096 50.3 / 46.1.
-// Nontemporal loads, us plain / nontemporal: 150 mixed streams to 8192 keys
-// (16 / 2 x 128) 113 / 103, 48 to 8192 (12 x 64) 159 / 145; 32768 keys of one
-// stream 19.7 / 20.3.
-constexpr int kManyUnits = 64;
-constexpr int64_t kFewBytes = int64_t(128) << 20;
+// Two forms (paged_index.h whole_units): workgroups of eight waves, one a CU,
+// whole ones a unit, so that a workgroup has one unit's chain of loads before it;
+// else of four waves, two a CU, in equal shares of all keys, with nontemporal loads.
+// Those, us plain / nontemporal: 150 mixed streams to 8192 keys (16 / 2 x 128) 113 /
+// 103, 48 to 8192 (12 x 64) 159 / 145; 32768 keys of one stream 19.7 / 20.3.
 // Equal shares: a unit counts kStart4 tiles on top of its own, about what its
 // chain of loads before the first tile and the meeting after the last cost, and
 // none is cut within kSlack of its ends.  us without / with: 128 mixed streams
@@ -573,7 +565,7 @@ void launch_paged_attn(const PagedAttn &a, float *work, unsigned *cnt, hipStream
   const int64_t units = static_cast<int64_t>(a.kv.batch) * a.kv.hkv * p.blocks;
   XE_REQUIRE(cap / kTile * units < (int64_t(1) << 31), "paged attention: more than 2^31 blocks of 16 keys in the table");
   const int64_t span = a.window ? std::min<int64_t>(cap, static_cast<int64_t>(a.window) + kTile) : cap;
-  const bool wide = a.kv.batch <= 64 && units <= gdev::cu_count() && (units < kManyUnits || units * span * a.kv.hd * 4 <= kFewBytes);
+  const bool wide = paged::whole_units(a.kv.batch, units, span, a.kv.hd, gdev::cu_count());
   const int kw = wide ? 8 : 4;
   const int64_t wgs = std::max<int64_t>(1, std::min<int64_t>(std::min(kMaxWg, (wide ? 1 : 2) * gdev::cu_count()), cap / kTile * units));
   const size_t lds = area_bytes(a.kv.hd, p.rows, kw) + 8 * static_cast<size_t>(a.kv.batch);

@@ -78,6 +78,25 @@ XE_HD unsigned least_share(unsigned longest, unsigned group, unsigned alone, uns
   return q <= more ? (q < more / 3 ? more / 3 : q) : 1;
 }
 
+// Whether units get whole workgroups, else equal shares: up to 64 streams (a lane
+// of a wave each) of up to a unit a CU, of fewer than kManyUnits units or of keys
+// (`span` a unit: what the table or the window allows) up to kFewBytes.  us in
+// whole workgroups / in shares: 32768 keys of one stream (4 x 256) 18.2 / 23.6, 8
+// mixed streams to 3000 keys (8 / 2 x 128) 9.7 / 10.8, 32 of window 1024 12.5 /
+// 16.5, 60 to 300 keys (16 / 4 x 128) 9.4 / 13.6, 64 to 1500 (4 x 256) 20.9 / 26.5,
+// 64 to 4096 50.3 / 46.1.  8, 16, 32, 48 and 63 streams of one length (4 / 1 x 256):
+//    64 MB   22.0 / 25.6  19.2 / 26.6  19.4 / 24.8  19.7 / 23.6  19.6 / 25.5
+//   150 MB   34.0 / 39.6  32.0 / 39.0  32.2 / 35.9  32.9 / 36.4  33.2 / 37.0
+//   300 MB   62.1 / 59.7  59.2 / 61.6  59.4 / 59.7  60.0 / 58.8  59.9 / 59.7
+//   500 MB   95.8 / 88.6  93.1 / 89.4  93.5 / 89.8  92.7 / 87.6  93.3 / 88.0
+// (mixed lengths and 8 / 2 and 32 / 8 x 128 alike): by bytes the two meet at about
+// 250 MB, and fewer than kManyUnits units beyond that are up to 8 % slower so.
+constexpr int kManyUnits = 64;
+constexpr int64_t kFewBytes = int64_t(128) << 20;
+inline bool whole_units(int batch, int64_t units, int64_t span, int hd, int cus) {
+  return batch <= 64 && units <= cus && (units < kManyUnits || units * span * hd * 4 <= kFewBytes);
+}
+
 // Shares begin at i * per, or at the end of a unit that lies at most `slack`
 // granules from there: neither a unit of few granules nor an end of one is
 // split off for its sake.  g lies in a unit of n granules of the stream that

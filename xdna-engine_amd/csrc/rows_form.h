@@ -1,4 +1,5 @@
-// rows_form.h -- which form of the int8 rows' product a shape takes.
+// rows_form.h -- on which way an int8 linear's rows become codes, and which form
+// of the product a shape takes.
 #pragma once
 
 #include <cstddef>
@@ -39,6 +40,26 @@ constexpr Form kForm[kForms] = {
     {128, 64, 128, 1, 3.44f, 0.305f, 0.219f, 1.72f},  {128, 128, 128, 1, 4.41f, 0.434f, 0.558f, 1.43f},
     {256, 128, 128, 1, 6.85f, 0.682f, 0.682f, 2.12f}, {16, 16, 256, 4, 4.28f, 0.185f, 0.139f, 49.2f},
     {16, 32, 256, 4, 4.28f, 0.230f, 0.188f, 21.2f}};
+
+// Codes and product in one launch or in two; rows off 16 bytes, and results that
+// lie over other workgroups' inputs, always take two.
+// One row of K up to kFusedK: each workgroup makes the codes for itself, behind its
+// first weight loads.  us in one launch / in two: 768 -> 768 4.4 / 6.2, 4096 ->
+// 4096 7.4 / 9.0, 1152 -> 13824 7.5 / 10.6.  Two rows one after the other took
+// longer than two launches where K is 4096.  32 weight rows a workgroup / 16: those
+// 4.8 / 4.4, 8.9 / 7.4, 7.5 / 8.2; 2048 -> 9000 8.6 / 8.4.
+// Up to kManyRows rows, a wave each, where that is one tile a CU.  us in one launch /
+// in two, 2 and 8 rows: 768 -> 1536 5.4 / 6.8, 5.4 / 6.9, 1152 -> 4096 6.6 / 7.1,
+// 6.6 / 7.4; 1600 -> 4096 7.6 / 7.1, 7.4 / 7.3; 16 rows on sixteen waves 768 ->
+// 1536 7.0 / 6.4, 256 -> 1536 6.4 / 6.2; four tiles a CU, 1152 -> 13824, 20 / 8.8.
+// One row so: 768 -> 1536 5.3, on all its workgroup's threads 4.6.
+constexpr int kFusedK = 4096;
+constexpr int kManyRows = 8, kManyK = 1280;
+enum Way { kOneRow, kOneRowWide, kWaveRows, kTwoLaunches };
+inline Way way(int m, int k, int batch, int cus) {
+  if (batch == 1 && k <= kFusedK) return m > 32 * cus ? kOneRowWide : kOneRow;
+  return batch <= kManyRows && m <= 16 * cus && k <= kManyK ? kWaveRows : kTwoLaunches;
+}
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 

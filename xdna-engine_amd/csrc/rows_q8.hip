@@ -22,9 +22,7 @@ constexpr size_t kPartBytes = rowsform::kPartBytes;  // partial tiles of K split
 constexpr size_t kCntWords = rowsform::kTiles;       // and their arrival counters
 constexpr int kMaxSplit = 4;        // parts of K
 constexpr int kStep = 128;          // bytes of K a step
-constexpr int kManyRows = 8;       // rows that its eight waves make, one each
-constexpr int kManyK = 1280;       // K up to which they do
-constexpr int kFusedK = 4096;       // K up to which a workgroup makes one row's codes itself
+constexpr int kFusedK = rowsform::kFusedK;
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
@@ -781,24 +779,15 @@ int launch_rows_q8(const RowsQ8 &L, hipStream_t s) {
   r.vec = ((rows_at & (r.a.act == XE_ACT_GEGLU ? 7 : 15)) | (weights_at & 15)) == 0;
   const bool in16 = ((reinterpret_cast<uintptr_t>(r.a.x) | reinterpret_cast<uintptr_t>(r.a.add) | reinterpret_cast<uintptr_t>(r.a.sum) |
                       reinterpret_cast<uintptr_t>(r.a.post_w)) & 15) == 0;
-  // One launch for one row: each workgroup makes the codes for itself, behind its
-  // first weight loads.  us in one launch / in two: 768 -> 768 4.4 / 6.2, 4096 ->
-  // 4096 7.4 / 9.0, 1152 -> 13824 7.5 / 10.6.  Two rows one after the other took
-  // longer than two launches where K is 4096.
-  if (in16 && r.a.batch == 1 && r.k <= kFusedK && !shares(r, outs)) {
-    // 32 weight rows a workgroup / 16: those 4.8 / 4.4, 8.9 / 7.4, 7.5 / 8.2; 2048 -> 9000 8.6 / 8.4
-    const bool wide = r.m > 32 * gdev::cu_count();
+  const rowsform::Way way = in16 && !shares(r, outs) ? rowsform::way(r.m, r.k, r.a.batch, gdev::cu_count()) : rowsform::kTwoLaunches;
+  if (way == rowsform::kOneRow || way == rowsform::kOneRowWide) {
+    const bool wide = way == rowsform::kOneRowWide;
     if (r.k <= 1024) wide ? launch_gemm<2, 1, 4, 4, 1>(r, 1, s) : launch_gemm<1, 1, 4, 8, 1>(r, 1, s);
     else if (r.k <= 2048) wide ? launch_gemm<2, 1, 4, 4, 2>(r, 1, s) : launch_gemm<1, 1, 4, 8, 2>(r, 1, s);
     else wide ? launch_gemm<2, 1, 4, 4, 4>(r, 1, s) : launch_gemm<1, 1, 4, 8, 4>(r, 1, s);
     return 1;
   }
-  // Up to eight rows, a wave each, where that is one tile a CU.  us in one launch /
-  // in two, 2 and 8 rows: 768 -> 1536 5.4 / 6.8, 5.4 / 6.9, 1152 -> 4096 6.6 / 7.1,
-  // 6.6 / 7.4; 1600 -> 4096 7.6 / 7.1, 7.4 / 7.3; 16 rows on sixteen waves 768 ->
-  // 1536 7.0 / 6.4, 256 -> 1536 6.4 / 6.2; four tiles a CU, 1152 -> 13824, 20 / 8.8.
-  // One row so: 768 -> 1536 5.3, on all its workgroup's threads 4.6.
-  if (in16 && r.a.batch <= kManyRows && r.m <= 16 * gdev::cu_count() && r.k <= kManyK && !shares(r, outs)) {
+  if (way == rowsform::kWaveRows) {
     if (r.k <= 768) launch_gemm<1, 1, 8, 2, 3, true>(r, 1, s);
     else launch_gemm<1, 1, 8, 3, 5, true>(r, 1, s);
     return 1;
